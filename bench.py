@@ -474,13 +474,21 @@ def run_reference(args, budget_s=150.0):
     # the C restatement parallelises inside (OpenMP); the reference runs one
     # thread per process
     procs = max(1, min(avail, args.steps)) if kind == "reference" else 1
-    ctx = mp.get_context("fork")
-    ready, go = ctx.Barrier(procs + 1), ctx.Barrier(procs + 1)
-    deadline = ctx.Value("d", 0.0)
-    out = ctx.Queue()
+    if kind == "reference":
+        ctx = mp.get_context("fork")
+        Worker, Barrier, out, deadline = ctx.Process, ctx.Barrier, ctx.Queue(), ctx.Value("d", 0.0)
+    else:
+        # one worker, a thread: a process forked after the warm-up would wait
+        # for ever on the OpenMP threads that only its parent has
+        import queue
+        import threading
+        import types
+        Worker, Barrier, out, deadline = (threading.Thread, threading.Barrier, queue.Queue(),
+                                          types.SimpleNamespace(value=0.0))
+    ready, go = Barrier(procs + 1), Barrier(procs + 1)
     quotas = [args.steps // procs + (1 if p < args.steps % procs else 0) for p in range(procs)]
-    ws = [ctx.Process(target=_ref_worker, args=(kind, eng, L, xs[p % 4:] + xs[:p % 4], quotas[p], deadline,
-                                                 ready, go, out)) for p in range(procs)]
+    ws = [Worker(target=_ref_worker, args=(kind, eng, L, xs[p % 4:] + xs[:p % 4], quotas[p], deadline,
+                                           ready, go, out)) for p in range(procs)]
     for w in ws:
         w.start()
     ready.wait()

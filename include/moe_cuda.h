@@ -56,8 +56,10 @@ typedef struct {
 #define MOE_ERR_NOMEM        6  /* device allocation failed */
 
 #define MOE_DTYPE_F32 0   /* unquantised fp32 experts (moe_cuda_upload_layer_f32) */
+#define MOE_DTYPE_F16 1   /* element types of the attention entry points */
 #define MOE_DTYPE_Q8 2
 #define MOE_DTYPE_Q4 3
+#define MOE_DTYPE_BF16 4
 
 /* moe_ffn flags */
 #define MOE_FFN_HOST_PTRS   0x1 /* x/out/topk pointers are host memory: the
@@ -327,6 +329,125 @@ int moe_cuda_ep_setup(int max_tokens_local, int D, int top_k, void* ipc_handle_o
 int moe_cuda_ep_connect(const void* ipc_handles);
 int moe_ffn_ep(int layer, const float* x_norm2, int T_local, float* x_inout,
                void* stream);
+
+/* ---- attention over a paged key-value cache ---------------------------------
+ * The part of a decode step that the reference runs on the CPU beside the MoE
+ * block (test_model_trace.c:341-445), on the GPU: a plan of the step's cache
+ * rows from the sequences' lengths, the per-head norm and rotation with the
+ * append to the cache, and the attention of each new row over its sequence's
+ * pages. All pointers are device memory, all calls are asynchronous on
+ * `stream` and may be captured into a CUDA graph; none needs moe_cuda_init.
+ * A call runs on the device that holds its first operand, whichever device is
+ * current (the stream must be that device's). The calls keep nothing between
+ * them: what they need beyond their operands is the caller's workspace.
+ *
+ * A cache of n_pages pages of page_size tokens of n_kv heads. Element strides;
+ * the head_dim elements of one head are contiguous. k and v 16-byte aligned,
+ * strides multiples of 16 bytes, head_dim a multiple of 8 up to 256
+ * (MOE_ERR_UNSUPPORTED otherwise), dtype MOE_DTYPE_F32, _F16 or _BF16.
+ * Slot s of the cache is token s % page_size of page s / page_size. */
+typedef struct {
+  void *k, *v;
+  int dtype;
+  int n_pages, page_size, n_kv, head_dim;
+  long long page_stride, token_stride, head_stride;
+} MoeKvCache;
+
+/* moe_kv_plan_dev: sequence s holds past_len[s] tokens (NULL: none) and gets
+ * new_len[s] more (lengths below 0 count as 0, and a sum stops at 2^31 - 1).
+ * It owns entries 0 .. ceil(past/page_size) - 1 of its row block_table[s]
+ * (max_pages entries). The call
+ *   - takes the pages that the new tokens need from the free list
+ *     free_pages[*free_head .. n_free), in the order of the sequences, and
+ *     writes them to the rows' next entries (-1 when the list is used up;
+ *     a sequence gets no pages past max_pages); other entries stay;
+ *   - numbers the new tokens as rows, sequence after sequence: row_seq (the
+ *     sequence), row_pos (the position in it) and row_slot (the slot of the
+ *     cache, -1 if its page is missing or not in [0, n_pages)). The rows from
+ *     the last new token to row_cap are padding: -1 in all three. New tokens
+ *     beyond row_cap get no row;
+ *   - kv_len[s] = past_len[s] + new_len[s], free_head_out = the first page not
+ *     taken, status[0..2] = rows asked for, pages asked for, pages taken.
+ *     Each of the three may be NULL; kv_len may be past_len and free_head_out
+ *     may be free_head, so that a captured step can be replayed.
+ * free_head may be NULL (0). At most 16384 sequences. */
+int moe_kv_plan_dev(const int* past_len, const int* new_len, int n_seq,
+                    int page_size, int n_pages, const int* free_pages, int n_free,
+                    const int* free_head, int* block_table, int max_pages,
+                    int* kv_len, int* row_seq, int* row_pos, int* row_slot,
+                    int row_cap, int* free_head_out, int* status, void* stream);
+
+/* moe_qk_norm_rope_dev: for each of `rows` rows, RMSNorm every query head
+ * (weights q_norm[head_dim]) and key head (k_norm; NULL: no norm), rotate them
+ * by row_pos, write the queries to q_out and append the row's keys and values
+ * to the cache at row_slot (test_model_trace.c:357-392). The rotation pairs
+ * elements i and i + rot_dim/2 for i < rot_dim/2; rope[p] holds the rot_dim/2
+ * cosines, then the rot_dim/2 sines of position p < rope_len; elements from
+ * rot_dim on pass through; rot_dim = 0 rotates nothing (row_pos may then be
+ * NULL). Computed in fp32, each output rounded once.
+ * q [rows][n_q][head_dim] with ldq elements from row to row, k and v
+ * [rows][n_kv][head_dim] with ldk, ldv: slices of one packed projection will
+ * do. dtype is their type; q_out (row stride ldo) and the cache have the
+ * cache's type, which for 16-bit rows must be the same and for fp32 rows may
+ * be any. q_out may be q, with the same type and stride; it must not overlap
+ * q, k or v otherwise. n_q may be 0 (keys and values only), row_slot NULL
+ * (queries only). A row whose position is negative or not below rope_len is
+ * padding: nothing of it is read or written. A slot outside the cache appends
+ * nothing. Rows must have different slots. */
+int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k, long long ldk,
+                         const void* v, long long ldv, int dtype, int rows, int n_q,
+                         const float* q_norm, const float* k_norm, float eps,
+                         const float* rope, int rot_dim, int rope_len,
+                         const int* row_pos, const int* row_slot, void* q_out,
+                         long long ldo, const MoeKvCache* cache, void* stream);
+
+/* moe_paged_attention_dev: out = softmax(scale * q k^T) v of every query head
+ * of every row over positions 0 .. row_pos of the row's sequence
+ * (test_model_trace.c:394-420); query head h reads key-value head
+ * h / (n_q / n_kv). row_seq[i] is row i's row of block_table[n_seq][max_pages]
+ * (NULL: row i of the table). q and out have the cache's type, ldq and ldo
+ * elements from row to row; out may be q (same stride). lse [rows][n_q]
+ * (NULL to skip): the natural logarithm of the softmax's sum, scale included.
+ *   - row_seq outside [0, n_seq): padding, the row of out and lse stays as it is.
+ *   - row_pos negative: no position; out is 0, lse -inf (also when every score
+ *     is -inf).
+ *   - Positions past max_pages * page_size and positions on a page outside
+ *     [0, n_pages) are not attended. Slots past row_pos are never read,
+ *     whatever they hold.
+ * max_kv is what the longest row is expected to hold; it only sets how far a
+ * row is split over the GPU (a longer row is right, but slower).
+ * workspace: moe_paged_attention_workspace() bytes (0: none needed), 16-byte
+ * aligned, no initial contents, one per call in flight: calls on two streams,
+ * or two graphs that may run at the same time, need one each. */
+size_t moe_paged_attention_workspace(int rows, int n_q, const MoeKvCache* cache,
+                                     int max_kv);
+int moe_paged_attention_dev(const void* q, long long ldq, const MoeKvCache* cache,
+                            const int* block_table, int n_seq, int max_pages,
+                            const int* row_seq, const int* row_pos, int rows, int n_q,
+                            int max_kv, float scale, void* out, long long ldo,
+                            float* lse, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* ---- expert routing from given logits ---------------------------------------
+ * moe_route_dev: topk_idx/topk_p [rows][top_k], the lists that moe_ffn takes
+ * with MOE_FFN_GIVEN_TOPK, from router logits [rows][E] (dtype MOE_DTYPE_F32,
+ * _F16 or _BF16, ld elements from row to row). The score s of an expert is the
+ * softmax over all E or the sigmoid of its logit. Experts are chosen by
+ * s + bias (bias [E], NULL: none), the largest first, equal ones by the lower
+ * index. n_group > 1: of the n_group equal groups of consecutive experts, only
+ * the keep_group with the largest sum of their best group_top (1 or 2) values
+ * are chosen from. The weight is s, without the bias, divided by the sum of
+ * the chosen (renorm != 0), times factor. Scores and choices are held in
+ * 64 bits. An expert whose logit is NaN or -inf, or whose bias is, is never
+ * chosen; where fewer than top_k are left, the index is -1 and the weight 0.
+ * E up to 1024, n_group and top_k up to 32. Device pointers, asynchronous, no
+ * moe_cuda_init needed. */
+#define MOE_ROUTE_SOFTMAX 0
+#define MOE_ROUTE_SIGMOID 1
+int moe_route_dev(const void* logits, long long ld, int dtype, int rows, int E,
+                  const float* bias, int score, int n_group, int keep_group,
+                  int group_top, int top_k, int renorm, double factor,
+                  int* topk_idx, float* topk_p, void* stream);
 
 /* ---- profiling -------------------------------------------------------------
  * Per-kernel device time of moe_ffn / moe_ffn_partial (CUDA events recorded

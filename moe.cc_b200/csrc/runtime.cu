@@ -51,8 +51,12 @@ static int set_err(int code, const char* fmt, ...) {
   return code;
 }
 
-// Error reporting for entry points defined in other .cu files of the library.
-int set_error_message(int code, const char* msg) { return set_err(code, "%s", msg); }
+// Error reporting for entry points defined in other .cu files of the library
+// (some of them take no lock otherwise, so this takes it).
+int set_error_message(int code, const char* msg) {
+  std::lock_guard<std::recursive_mutex> lk(g.mu);
+  return set_err(code, "%s", msg);
+}
 
 #define CU(call)                                                                         \
   do {                                                                                   \

@@ -23,7 +23,8 @@ MOE_ERR_RANGE, MOE_ERR_UNSUPPORTED, MOE_ERR_NOMEM = 4, 5, 6
 Q8, Q4 = 2, 3
 HOST_PTRS, DEVICE_PTRS, FORCE_GEMV, FORCE_GEMM = 0x1, 0x0, 0x4, 0x8
 SEQ_RESIDUAL, GIVEN_TOPK = 0x10, 0x20
-F32 = 0
+F32, F16, BF16 = 0, 1, 4
+ROUTE_SCORES = {"softmax": 0, "sigmoid": 1}
 
 # Every symbol include/moe_cuda.h declares (checked by the CPU test suite).
 EXPORTS = (
@@ -41,6 +42,8 @@ EXPORTS = (
     "moe_bin_layer_info_h", "moe_cuda_load_bin_layer_h",
     "moe_bin_create", "moe_bin_put", "moe_bin_finish",
     "moe_quantize_rowwise_q8_host", "moe_quantize_rowwise_q4_host",
+    "moe_kv_plan_dev", "moe_qk_norm_rope_dev", "moe_paged_attention_workspace", "moe_paged_attention_dev",
+    "moe_route_dev",
 )
 
 
@@ -56,6 +59,13 @@ class QuantizedWeight(C.Structure):
                 ("cols", C.c_int), ("dtype", C.c_int)]
 
 
+class MoeKvCache(C.Structure):
+    """A paged key-value cache (include/moe_cuda.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("n_kv", C.c_int), ("head_dim", C.c_int),
+                ("page_stride", C.c_longlong), ("token_stride", C.c_longlong), ("head_stride", C.c_longlong)]
+
+
 _lib = None
 
 
@@ -67,6 +77,7 @@ def lib():
             raise MoeError(MOE_ERR_NOT_INIT, f"{LIB_PATH} is not built (run make -C moe.cc_b200)")
         L = C.CDLL(LIB_PATH)
         vp, i, sz, u64, f = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_float
+        ll, d = C.c_longlong, C.c_double
         sig = {
             "moe_cuda_init": ([i, i, i, vp], i), "moe_cuda_shutdown": ([], i),
             "moe_cuda_last_error": ([], C.c_char_p), "moe_cuda_check_status": ([], i),
@@ -105,6 +116,11 @@ def lib():
             "moe_bin_finish": ([vp], i),
             "moe_quantize_rowwise_q8_host": ([vp, i, i, vp, vp], i),
             "moe_quantize_rowwise_q4_host": ([vp, i, i, vp, vp], i),
+            "moe_kv_plan_dev": ([vp, vp, i, i, i, vp, i, vp, vp, i, vp, vp, vp, vp, i, vp, vp, vp], i),
+            "moe_qk_norm_rope_dev": ([vp, ll, vp, ll, vp, ll, i, i, i, vp, vp, f, vp, i, i, vp, vp, vp, ll, vp, vp], i),
+            "moe_paged_attention_workspace": ([i, i, vp, i], sz),
+            "moe_paged_attention_dev": ([vp, ll, vp, vp, i, i, vp, vp, i, i, i, f, vp, ll, vp, vp, sz, vp], i),
+            "moe_route_dev": ([vp, ll, i, i, i, vp, i, i, i, i, i, i, d, vp, vp, vp], i),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)
@@ -385,6 +401,152 @@ def moe_ffn_ep(layer, x_norm2, x_inout, stream=None):
     """Expert-parallel MoE block over this rank's tokens, exchanges fused into
     the kernels (include/moe_cuda.h: moe_ffn_ep)."""
     check(lib().moe_ffn_ep(layer, _p(x_norm2), x_inout.shape[0], _p(x_inout), _stream(stream)))
+
+
+# ---- attention over a paged key-value cache, expert routing ------------------
+# torch CUDA tensors; `stream` as in the calls above. A tensor of the wrong type,
+# place or layout is refused here, before its pointer is handed on.
+
+_ELEM = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+
+
+def _elem(t, what):
+    d = _ELEM.get(str(t.dtype))
+    if d is None:
+        raise MoeError(MOE_ERR_INVALID, f"{what}: float32, float16 or bfloat16 is wanted, got {t.dtype}")
+    return d
+
+
+def _dev(t, kind, shape, what, device):
+    """Pointer of a contiguous device tensor of the given type and shape (None: any length); None passes through."""
+    if t is None:
+        return None
+    if str(t.dtype) != kind or not t.is_contiguous() or t.device != device or t.dim() != len(shape) or any(
+            n is not None and m != n for m, n in zip(t.shape, shape)):
+        raise MoeError(MOE_ERR_INVALID, f"{what}: a contiguous {kind} tensor of shape {shape} on {device} is wanted, "
+                                        f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(t, what, heads, hd, device):
+    """(pointer, row stride) of [rows][heads][head_dim] whose rows may lie apart."""
+    if t.dim() != 3 or t.device != device or t.shape[2] != hd or (heads is not None and t.shape[1] != heads) or (
+            t.numel() and ((hd > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != hd))):
+        raise MoeError(MOE_ERR_INVALID, f"{what}: [rows][heads][{hd}] on {device} with contiguous rows is wanted, "
+                                        f"got {tuple(t.shape)}, strides {t.stride()} on {t.device}")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1] * hd)
+
+
+def _cuda_device(t, what):
+    if not t.is_cuda:
+        raise MoeError(MOE_ERR_INVALID, f"{what}: a CUDA tensor is wanted")
+    return t.device
+
+
+def kv_cache(k, v):
+    """MoeKvCache of two tensors [n_pages][page_size][n_kv][head_dim] of one
+    type and one layout, the last dimension contiguous, the others in any
+    order. The tensors must outlive it."""
+    shape, sk, sv = k.shape, k.stride(), v.stride()
+    if len(shape) == 4 and 1 in shape and sk != sv:          # the stride of a dimension of one says nothing
+        sk, sv = ([0 if n == 1 else s for n, s in zip(shape, st)] for st in (sk, sv))
+    if len(shape) != 4 or shape != v.shape or k.dtype != v.dtype or sk != sv or k.device != v.device:
+        raise MoeError(MOE_ERR_INVALID, "kv cache: k and v of one type and layout, [n_pages][page_size][n_kv][head_dim]")
+    n, ps, nkv, hd = shape
+    if hd > 1 and sk[3] != 1:
+        raise MoeError(MOE_ERR_INVALID, "kv cache: the head dimension must be contiguous")
+    return MoeKvCache(k.data_ptr(), v.data_ptr(), _elem(k, "kv cache"), n, ps, nkv, hd, sk[0], sk[1], sk[2])
+
+
+def kv_plan(past_len, new_len, page_size, n_pages, free_pages, block_table, row_seq, row_pos, row_slot, kv_len=None,
+            free_head=None, free_head_out=None, status=None, stream=None):
+    """moe_kv_plan_dev: int32 tensors; past_len may be None (nothing held yet)."""
+    n, mp = block_table.shape
+    dev, cap, i32 = _cuda_device(block_table, "kv_plan"), row_seq.shape[0], "torch.int32"
+    check(lib().moe_kv_plan_dev(
+        _dev(past_len, i32, (n,), "past_len", dev), _dev(new_len, i32, (n,), "new_len", dev), n, page_size, n_pages,
+        _dev(free_pages, i32, (None,), "free_pages", dev), free_pages.shape[0], _dev(free_head, i32, (1,), "free_head", dev),
+        _dev(block_table, i32, (n, mp), "block_table", dev), mp, _dev(kv_len, i32, (n,), "kv_len", dev),
+        _dev(row_seq, i32, (cap,), "row_seq", dev), _dev(row_pos, i32, (cap,), "row_pos", dev),
+        _dev(row_slot, i32, (cap,), "row_slot", dev), cap, _dev(free_head_out, i32, (1,), "free_head_out", dev),
+        _dev(status, i32, (3,), "status", dev), _stream(stream)))
+
+
+def qk_norm_rope(q, k, v, k_cache, v_cache, row_pos, row_slot, q_out, rope=None, q_norm=None, k_norm=None, eps=1e-6,
+                 stream=None):
+    """moe_qk_norm_rope_dev. q [rows][n_q][head_dim] (None: keys and values
+    only), k, v [rows][n_kv][head_dim], rows of one stride each; rope
+    [positions][rot_dim] fp32, the cosines then the sines; row_slot None:
+    queries only (k, v are then not read and may be None)."""
+    c = kv_cache(k_cache, v_cache)
+    hd, dev, i32, f32 = c.head_dim, _cuda_device(k_cache, "qk_norm_rope"), "torch.int32", "torch.float32"
+    x = q if q is not None else k
+    rows, dt = x.shape[0], _elem(x, "q")
+    qp = op = kp = vp = None
+    ldq = ldo = ldk = ldv = n_q = 0
+    if q is not None:
+        n_q = q.shape[1]
+        qp, ldq = _rows(q, "q", n_q, hd, dev)
+        op, ldo = _rows(q_out, "q_out", n_q, hd, dev)
+        if q_out.dtype != k_cache.dtype or q_out.shape[0] != rows:
+            raise MoeError(MOE_ERR_INVALID, "q_out: the rows of q in the cache's type are wanted")
+    if row_slot is not None:
+        kp, ldk = _rows(k, "k", c.n_kv, hd, dev)
+        vp, ldv = _rows(v, "v", c.n_kv, hd, dev)
+        if k.dtype != x.dtype or v.dtype != x.dtype or k.shape[0] != rows or v.shape[0] != rows:
+            raise MoeError(MOE_ERR_INVALID, "q, k and v: one type and one number of rows")
+    rot, n_rope = (rope.shape[1], rope.shape[0]) if rope is not None else (0, 0)
+    check(lib().moe_qk_norm_rope_dev(
+        qp, ldq, kp, ldk, vp, ldv, dt, rows, n_q, _dev(q_norm, f32, (hd,), "q_norm", dev),
+        _dev(k_norm, f32, (hd,), "k_norm", dev), eps, _dev(rope, f32, (n_rope, rot), "rope", dev), rot, n_rope,
+        _dev(row_pos, i32, (rows,), "row_pos", dev), _dev(row_slot, i32, (rows,), "row_slot", dev), op, ldo,
+        C.byref(c), _stream(stream)))
+
+
+def paged_attention_workspace(rows, n_q, k_cache, v_cache, max_kv):
+    """Bytes of workspace of a paged_attention call (0: none)."""
+    return lib().moe_paged_attention_workspace(rows, n_q, C.byref(kv_cache(k_cache, v_cache)), max_kv)
+
+
+def paged_attention(q, k_cache, v_cache, block_table, row_pos, out, workspace, max_kv, scale, lse=None, row_seq=None,
+                    stream=None):
+    """moe_paged_attention_dev. q, out [rows][n_q][head_dim]; workspace: a
+    contiguous tensor of any type (None where none is needed)."""
+    c = kv_cache(k_cache, v_cache)
+    dev, i32 = _cuda_device(k_cache, "paged_attention"), "torch.int32"
+    rows, n_q = q.shape[0], q.shape[1]
+    qp, ldq = _rows(q, "q", n_q, c.head_dim, dev)
+    op, ldo = _rows(out, "out", n_q, c.head_dim, dev)
+    if q.dtype != k_cache.dtype or out.dtype != k_cache.dtype or out.shape[0] != rows:
+        raise MoeError(MOE_ERR_INVALID, "q and out: the same rows in the cache's type are wanted")
+    n_seq, mp = block_table.shape
+    wp, wn = None, 0
+    if workspace is not None:
+        if not workspace.is_contiguous() or workspace.device != dev:
+            raise MoeError(MOE_ERR_INVALID, f"workspace: a contiguous tensor on {dev} is wanted")
+        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    check(lib().moe_paged_attention_dev(
+        qp, ldq, C.byref(c), _dev(block_table, i32, (n_seq, mp), "block_table", dev), n_seq, mp,
+        _dev(row_seq, i32, (rows,), "row_seq", dev), _dev(row_pos, i32, (rows,), "row_pos", dev), rows, n_q, max_kv, scale,
+        op, ldo, _dev(lse, "torch.float32", (rows, n_q), "lse", dev), wp, wn, _stream(stream)))
+
+
+def route(logits, topk_idx, topk_p, bias=None, score="softmax", groups=1, keep_groups=1, group_top=1, renorm=True,
+          scale=1.0, stream=None):
+    """moe_route_dev: topk_idx (int32) and topk_p (fp32) [rows][top_k] of
+    logits [rows][E] (rows may lie apart)."""
+    dev = _cuda_device(logits, "route")
+    T, E = logits.shape
+    if T and E > 1 and logits.stride(1) != 1:
+        raise MoeError(MOE_ERR_INVALID, "logits: the experts must be contiguous")
+    if score not in ROUTE_SCORES:
+        raise MoeError(MOE_ERR_INVALID, f"score: one of {sorted(ROUTE_SCORES)} is wanted")
+    k = topk_idx.shape[1]
+    check(lib().moe_route_dev(
+        logits.data_ptr(), logits.stride(0) if T > 1 else E, _elem(logits, "logits"), T, E,
+        _dev(bias, "torch.float32", (E,), "bias", dev), ROUTE_SCORES[score], groups, keep_groups, group_top, k,
+        int(bool(renorm)), scale, _dev(topk_idx, "torch.int32", (T, k), "topk_idx", dev),
+        _dev(topk_p, "torch.float32", (T, k), "topk_p", dev), _stream(stream)))
 
 
 def profile(enable):

@@ -63,9 +63,10 @@ class OnDeviceOf {
   int back_ = -1, dev_ = 0;
 };
 
-inline int launched(const char* who) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? MOE_OK : fail(MOE_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+inline int launched(cudaError_t e, const char* who) {
+  if (e == cudaSuccess) return MOE_OK;
+  cudaGetLastError();
+  return fail(MOE_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }
 
 // The cache description every entry point that touches it checks alike.

@@ -61,6 +61,8 @@ __device__ __forceinline__ double sigmoid64(float x) { return 1.0 / (1.0 + exp(-
 // EPL experts a lane; SCORED: the choice needs every score (bias or groups)
 template <typename T, int EPL, bool SCORED>
 __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteArgs a) {
+  pdl_wait();
+  pdl_launch();
   extern __shared__ double choice_sm[];                    // groups: [kWarps][EPL * 32]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = (long long)blockIdx.x * kWarps + warp;
@@ -192,22 +194,22 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
 }
 
 template <typename T, int EPL>
-void launch_route_epl(const RouteArgs& a, bool scored, cudaStream_t st) {
+cudaError_t launch_route_epl(const RouteArgs& a, bool scored, cudaStream_t st) {
   const unsigned grid = (unsigned)((a.rows + kWarps - 1) / kWarps);
   const size_t smem = a.groups > 1 ? sizeof(double) * kWarps * EPL * 32 : 0;
-  if (scored) expert_route_kernel<T, EPL, true><<<grid, kWarps * 32, smem, st>>>(a);
-  else expert_route_kernel<T, EPL, false><<<grid, kWarps * 32, 0, st>>>(a);
+  if (scored) return launch_pdl(expert_route_kernel<T, EPL, true>, dim3(grid), dim3(kWarps * 32), smem, st, a);
+  return launch_pdl(expert_route_kernel<T, EPL, false>, dim3(grid), dim3(kWarps * 32), 0, st, a);
 }
 
 template <typename T>
-void launch_route(const RouteArgs& a, bool scored, cudaStream_t st) {
+cudaError_t launch_route(const RouteArgs& a, bool scored, cudaStream_t st) {
   const int epl = (a.E + 31) / 32;
-  if (epl <= 1) launch_route_epl<T, 1>(a, scored, st);
-  else if (epl <= 2) launch_route_epl<T, 2>(a, scored, st);
-  else if (epl <= 4) launch_route_epl<T, 4>(a, scored, st);
-  else if (epl <= 8) launch_route_epl<T, 8>(a, scored, st);
-  else if (epl <= 16) launch_route_epl<T, 16>(a, scored, st);
-  else launch_route_epl<T, 32>(a, scored, st);
+  if (epl <= 1) return launch_route_epl<T, 1>(a, scored, st);
+  if (epl <= 2) return launch_route_epl<T, 2>(a, scored, st);
+  if (epl <= 4) return launch_route_epl<T, 4>(a, scored, st);
+  if (epl <= 8) return launch_route_epl<T, 8>(a, scored, st);
+  if (epl <= 16) return launch_route_epl<T, 16>(a, scored, st);
+  return launch_route_epl<T, 32>(a, scored, st);
 }
 
 }  // namespace
@@ -243,8 +245,7 @@ extern "C" int moe_route_dev(const void* logits, long long ld, int dtype, int ro
   while (2 * a.lanes_per_group * n_group <= 32) a.lanes_per_group *= 2;
   const bool scored = bias || a.groups > 1;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == MOE_DTYPE_F32) launch_route<float>(a, scored, st);
-  else if (dtype == MOE_DTYPE_BF16) launch_route<__nv_bfloat16>(a, scored, st);
-  else launch_route<__half>(a, scored, st);
-  return at::launched(who);
+  return at::launched(dtype == MOE_DTYPE_F32    ? launch_route<float>(a, scored, st)
+                      : dtype == MOE_DTYPE_BF16 ? launch_route<__nv_bfloat16>(a, scored, st)
+                                                : launch_route<__half>(a, scored, st), who);
 }

@@ -56,6 +56,8 @@ __device__ __forceinline__ int owner_of(const int* end, int n, int i) {
 }
 
 __global__ void __launch_bounds__(kMaxThreads) kv_plan_kernel(const PlanArgs a) {
+  pdl_wait();
+  pdl_launch();
   extern __shared__ int sm[];
   __shared__ int warp_rows[32], warp_pages[32];
   int *past = sm, *row_end = sm + a.n_seq, *page_end = sm + 2 * a.n_seq;
@@ -181,12 +183,19 @@ extern "C" int moe_kv_plan_dev(const int* past_len, const int* new_len, int n_se
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute cl[1];
-  cl[0].id = cudaLaunchAttributeClusterDimension;
-  cl[0].val.clusterDim.x = ctas; cl[0].val.clusterDim.y = cl[0].val.clusterDim.z = 1;
-  cfg.attrs = cl;
-  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  cudaLaunchAttribute attrs[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (ctas > 1) {
+    attrs[n].id = cudaLaunchAttributeClusterDimension;
+    attrs[n].val.clusterDim.x = ctas; attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attrs;
+  cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_plan_kernel, a);
-  if (e != cudaSuccess) { cudaGetLastError(); return at::fail(MOE_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e)); }
-  return MOE_OK;
+  return at::launched(e, who);
 }

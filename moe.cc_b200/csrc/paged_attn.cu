@@ -36,6 +36,8 @@
 // from zero per step and added to fp32 sums outside the tensor core.
 #include "attn.cuh"
 
+#include <float.h>
+
 #include <atomic>
 #include <type_traits>
 
@@ -43,7 +45,11 @@ namespace moe {
 namespace {
 
 constexpr int kMaxParts = 128;      // runs a row is split into at most
-constexpr int kMinRun = 64;         // positions of the shortest run
+constexpr int kPiece = 64;          // positions of the shortest run
+constexpr int kDealtRows = 512;     // rows whose work is dealt evenly
+constexpr int kShort = 32;          // pieces up to which a cluster takes a row
+constexpr int kCluster = 8;         // CTAs of such a cluster at most
+enum { kRuns = 0, kDealt = 1, kClustered = 2 };
 constexpr int kStep = 16;           // positions a warp takes at a time
 constexpr float kRaise = 8.0f;      // log2 by which a score may exceed the reference
 
@@ -54,28 +60,31 @@ struct AttnArgs {
   float *lse, *part_o;
   float2* part_ml;
   long long ldq, ldo, page_stride, token_stride, head_stride, capacity;
-  int rows, n_q, n_kv, group, hd, tiles, n_seq, n_pages, page_size, max_pages, parts;
+  int rows, n_q, n_kv, group, hd, tiles, n_seq, n_pages, page_size, max_pages;
+  int parts;          // partial results that a row's head has room for
+  int mode;           // how the work is split (paged_attn_kernel)
   float scale_log2;
   at::FastDiv page;
 };
 
-// The runs of a row: how many, and how long each (a multiple of 64 so that
-// steps never straddle the start of a page that holds a multiple of 16).
-struct Runs { int len, run, n; };
-__device__ __forceinline__ Runs runs_of(int pos, long long capacity, int parts) {
-  Runs r;
-  r.len = pos < 0 ? 0 : (int)min((long long)pos + 1, capacity);
-  const int even = (r.len + parts - 1) / parts;
-  r.run = max(kMinRun, (even + 63) / 64 * 64);
-  r.n = r.len ? 1 + (r.len - 1) / r.run : 0;
-  return r;
+// Positions are dealt out in pieces of 64 (steps of 16 then never straddle the
+// start of a page that holds a multiple of 16).
+__device__ __forceinline__ int length_of(const AttnArgs& a, int row) {
+  const int seq = a.row_seq ? a.row_seq[row] : row;
+  if (seq < 0 || seq >= a.n_seq) return -1;                    // a padded row: left as it is
+  const int pos = a.row_pos[row];
+  return pos < 0 ? 0 : (int)min((long long)pos + 1, a.capacity);
 }
+__device__ __forceinline__ int pieces_of(int len) { return len > 0 ? (len - 1) / kPiece + 1 : 0; }
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool on) {
   const int n = on ? 16 : 0;        // 0: the 16 bytes are zeroed and src is not read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy16(unsigned dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -111,10 +120,10 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], const unsigned (&a)[4],
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo with hi a tf32 number (11 bits, nearest) and lo the fp32
-// remainder, of which the tensor core reads another 11 bits
+// x = hi + lo with hi the leading 11 bits of x, as a tf32 number holds them,
+// and lo the exact rest, of which the tensor core reads another 11 bits
 __device__ __forceinline__ void split_tf32(float x, unsigned& hi, unsigned& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  hi = __float_as_uint(x) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
@@ -140,131 +149,201 @@ template <> __device__ __forceinline__ void store1<__half>(void* p, long long i,
 
 // Shapes of one instantiation. HD: head_dim rounded up to 64, 128 or 256 (the
 // columns between are zeros in shared memory); NT: 8-head column tiles.
+#ifndef PA_W16
+#define PA_W16 4
+#endif
+#ifndef PA_U16
+#define PA_U16 3
+#endif
+#ifndef PA_C16
+#define PA_C16 2
+#endif
+#ifndef PA_W32
+#define PA_W32 (HD == 64 ? 8 : 4)
+#endif
+#ifndef PA_C32
+#define PA_C32 (HD == 128 ? 2 : 1)
+#endif
+#ifndef PA_U32
+#define PA_U32 3
+#endif
 template <typename T, int HD, int NT>
 struct Shape {
   static constexpr bool wide = sizeof(T) == 4;
-  // Row pitches that make the fragment loads conflict-free: 16-bit rows an odd
-  // number of 16-byte pieces (ldmatrix); fp32 K rows 16 words past a multiple
-  // of 32 (16-byte loads by 4 lanes of each of 2 rows), V rows 8 words past it
-  // (8-byte reach of 4 rows).
-  static constexpr int k_pitch = wide ? HD * 4 + 64 : HD * 2 + 16;
-  static constexpr int v_pitch = wide ? HD * 4 + 32 : HD * 2 + 16;
-  static constexpr int stage = kStep * (k_pitch + v_pitch);
-  // 16-bit up to 128: two CTAs of 4 warps on an SM; above, and fp32: one
-  static constexpr int warps = wide && HD == 256 ? 2 : 4;
-  static constexpr int stages = 3;
-  static constexpr int ctas = (wide ? HD <= 64 : HD <= 128) ? 2 : 1;
+  // A row's pitch keeps the fragment loads free of bank conflicts: 16-bit rows
+  // an odd number of 16-byte pieces (ldmatrix), fp32 rows 8 words past a
+  // multiple of 32 (16-byte loads of 2 rows two apart, or of 4 rows 8 words each).
+  static constexpr int pitch = wide ? HD * 4 + 32 : HD * 2 + 16;
+  static constexpr int unit = kStep * pitch;       // the K or the V rows of a step
+  static constexpr int warps = wide ? (HD == 256 ? 4 : PA_W32) : HD == 256 ? 8 : NT == 2 ? 4 : PA_W16;
+  static constexpr int units = wide ? (HD == 64 ? 5 : PA_U32) : HD == 256 ? 3 : NT == 2 || HD == 64 ? 5 : PA_U16;
+  static constexpr int ctas = wide ? PA_C32 : HD == 256 ? 1 : NT == 2 ? 2 : PA_C16;
   static constexpr int heads = 8 * NT;
-  static constexpr int q_bytes = wide ? 2 * heads * k_pitch : 0;      // fp32: Q's high and low parts
-  static constexpr int ring = warps * stages * stage;
+  static constexpr int q_pitch = HD * 4 + 64;      // fp32: Q's high and low parts, rows 16 words past
+  static constexpr int q_bytes = wide ? 2 * heads * q_pitch : 0;
+  static constexpr int ring = warps * units * unit;
   static constexpr int join = warps * heads * (HD + 2) * 4;
-  static constexpr int smem = (ring > join ? ring : join) + q_bytes + 64;
+  static constexpr int both = join + heads * (HD + 2) * 4;   // and the CTA's own result, for its cluster
+  static constexpr int base = ring > both ? ring : both;
+  static constexpr int smem = base + q_bytes;
 };
 
+// K row (position within the step) that matrix row g of the fp32 path holds:
+// g with its two lowest bits exchanged, so that the rows of one 16-byte load
+// phase lie two pitches apart
+__device__ __forceinline__ int swap01(int g) { return (g & 4) | ((g & 1) << 1) | ((g >> 1) & 1); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// what CTA `rank` of the cluster has at p in its shared memory
+__device__ __forceinline__ unsigned remote(const float* p, int rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 remote2(const float* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 remote4(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote(p, rank)) : "memory");
+  return v;
+}
+
+// Four elements of a row's result, and its lse with the first.
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnArgs& a, int row, int head, int d, float (&acc)[4], float sum, float m) {
+  using V = at::Vec4<T>;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] *= inv;
+  *reinterpret_cast<typename V::raw*>((T*)a.out + row * a.ldo + (long long)head * a.hd + d) = V::put(acc);
+  if (a.lse && d == 0) a.lse[(long long)row * a.n_q + head] = (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+// One run: positions [t0, t1) of one row for one tile of one key-value head's
+// query heads, `part` of `parts` such runs.
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(Shape<T, HD, NT>::warps * 32, Shape<T, HD, NT>::ctas)
-paged_attn_kernel(const AttnArgs a) {
+__device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int row, int kvh, int tile, int t0, int t1,
+                                       int part, int parts) {
   using S = Shape<T, HD, NT>;
-  extern __shared__ __align__(16) unsigned char sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, q4 = lane & 3;
-  // the small kernel that joins the runs may be scheduled from here on; it
-  // waits for this grid's end before it reads
-  pdl_launch();
-
-  const int part = blockIdx.x % a.parts;
-  int item = blockIdx.x / a.parts;
-  const int tile = item % a.tiles; item /= a.tiles;
-  const int kvh = item % a.n_kv, row = item / a.n_kv;
   const int seq = a.row_seq ? a.row_seq[row] : row;
-  if (seq < 0 || seq >= a.n_seq) return;                       // a padded row: left as it is
-  const int head0 = kvh * a.group + tile * S::heads;           // first query head of this CTA
+  const int head0 = kvh * a.group + tile * S::heads;           // first query head
   const int heads = min(S::heads, a.group - tile * S::heads);
-  const Runs rn = runs_of(a.row_pos[row], a.capacity, a.parts);
-  if (rn.n == 0) {                                             // no position: zeros
-    if (part == 0) {
-      for (int i = threadIdx.x; i < heads * a.hd; i += S::warps * 32) {
-        const int h = i / a.hd;
-        store1<T>(a.out, row * a.ldo + (long long)(head0 + h) * a.hd + (i - h * a.hd), 0.f);
-      }
-      if (a.lse && threadIdx.x < heads) a.lse[(long long)row * a.n_q + head0 + threadIdx.x] = -INFINITY;
-    }
-    return;
-  }
-  if (part >= rn.n) return;
-  const int t0 = part * rn.run, t1 = min(rn.len, t0 + rn.run);
   const int n_steps = (t1 - t0 + kStep - 1) / kStep;
   const int mine = n_steps > warp ? (n_steps - warp + S::warps - 1) / S::warps : 0;
 
-  unsigned char* ring = sm + warp * (S::stages * S::stage);
+  unsigned char* ring = sm + warp * (S::units * S::unit);
   const int* table = a.table + (long long)seq * a.max_pages;
-  const T* kbase = (const T*)a.k + kvh * a.head_stride;
-  const T* vbase = (const T*)a.v + kvh * a.head_stride;
   constexpr int kPieces = HD * (int)sizeof(T) / 16;            // 16-byte pieces of a row
   const int pieces = a.hd * (int)sizeof(T) / 16;
+  const char* kbase = (const char*)((const T*)a.k + kvh * a.head_stride);
+  const char* vbase = (const char*)((const T*)a.v + kvh * a.head_stride);
+  const long long row_bytes = a.token_stride * (long long)sizeof(T);
+  const bool whole = a.page_size % kStep == 0;                 // a step never leaves its page
 
   // columns from head_dim to HD are zeros throughout: no copy touches them
   if (pieces < kPieces) {
-    for (int i = lane; i < S::stages * 2 * kStep * (kPieces - pieces); i += 32) {
-      const int c = pieces + i % (kPieces - pieces), r = i / (kPieces - pieces) % kStep;
-      const int m = i / (kPieces - pieces) / kStep, st = m >> 1;
-      unsigned char* p = ring + st * S::stage + ((m & 1) ? kStep * S::k_pitch + r * S::v_pitch : r * S::k_pitch);
-      *reinterpret_cast<uint4*>(p + 16 * c) = make_uint4(0, 0, 0, 0);
-    }
+    const int pad = kPieces - pieces;
+    for (int i = lane; i < S::units * kStep * pad; i += 32)
+      *reinterpret_cast<uint4*>(ring + i / pad * S::pitch + 16 * (pieces + i % pad)) = make_uint4(0, 0, 0, 0);
   }
 
-  // Page of position `lane & 15` of step i, -1 where there is none; read one
-  // step before the copies that need it.
+  // Page of step i (of position `lane & 15` of it, where a step may span
+  // pages), -1 where there is none. Read one step before the copies need it.
   auto page_at = [&](int i) -> int {
-    const int t = t0 + (i * S::warps + warp) * kStep + (lane & 15);
+    const int t = t0 + (i * S::warps + warp) * kStep + (whole ? 0 : (lane & 15));
     if (i >= mine || t >= t1) return -1;
     return table[a.page.div((unsigned)t)];
   };
-  // valid positions of the stages in flight, two 16-bit masks a word
-  unsigned masks[S::stages];
-  auto issue = [&](int i, int pg, int st) -> unsigned {
+  // Copies the K or V rows of step i to a unit of the ring and returns the mask
+  // of the step's positions that are attended; the others' rows become zeros.
+  constexpr int kRows = kPieces <= 32 ? 32 / kPieces : 1;      // rows one instruction of the warp covers
+  constexpr int kInsn = kStep * kPieces / 32;
+  const int r0 = kPieces <= 32 ? lane / kPieces : 0, c0 = kPieces <= 32 ? lane % kPieces : lane;
+  auto issue = [&](const char* base, int i, int pg, int slot) -> unsigned {
     if (i >= mine) return 0u;
-    const int t = t0 + (i * S::warps + warp) * kStep + (lane & 15);
+    const int t = t0 + (i * S::warps + warp) * kStep;
     const bool ok = pg >= 0 && pg < a.n_pages;
-    long long off = 0;
-    if (ok) off = pg * a.page_stride + (t - (int)a.page.div((unsigned)t) * a.page_size) * a.token_stride;
-    const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
-    const unsigned kd = smem_u32(ring + st * S::stage), vd = kd + kStep * S::k_pitch;
+    const unsigned to = smem_u32(ring + slot * S::unit) + r0 * S::pitch + 16 * c0;
+    if (whole) {
+      const int n = ok ? min(kStep, t1 - t) : 0;
+      const int in = t - (int)a.page.div((unsigned)t) * a.page_size;
+      const char* src = base + (ok ? pg * a.page_stride * (long long)sizeof(T) + (in + r0) * row_bytes : 0) + 16 * c0;
+      if (n == kStep && (kPieces <= 32 || pieces == kPieces)) {   // the usual step: nothing to mask
+        if (c0 < pieces) {
 #pragma unroll
-    for (int j = 0; j < kStep * kPieces / 32; ++j) {
-      const int e = j * 32 + lane, r = e / kPieces, c = e % kPieces;
-      const long long o = __shfl_sync(~0u, off, r);
-      const bool on = (mask >> r) & 1;
-      if (c < pieces) {
-        copy16(kd + r * S::k_pitch + 16 * c, (const char*)(kbase + o) + 16 * c, on);
-        copy16(vd + r * S::v_pitch + 16 * c, (const char*)(vbase + o) + 16 * c, on);
+          for (int j = 0; j < kInsn; ++j) {
+            const int r = kPieces <= 32 ? j * kRows : j / 2, c = kPieces <= 32 ? 0 : 32 * (j & 1);
+            copy16(to + r * S::pitch + 16 * c, src + 16 * c);
+            if (kPieces <= 32 || (j & 1)) src += kRows * row_bytes;
+          }
+        }
+        return 0xffffu;
       }
+#pragma unroll 1
+      for (int j = 0; j < kInsn; ++j) {
+        const int r = kPieces <= 32 ? j * kRows : j / 2, c = kPieces <= 32 ? 0 : 32 * (j & 1);
+        if (c0 + c < pieces) copy16(to + r * S::pitch + 16 * c, src + r * row_bytes + 16 * c, r0 + r < n);
+      }
+      return (1u << n) - 1u;
+    }
+    const int tl = t + (lane & 15);
+    long long off = 0;
+    if (ok) off = pg * a.page_stride * (long long)sizeof(T) + (tl - (int)a.page.div((unsigned)tl) * a.page_size) * row_bytes;
+    const unsigned mask = __ballot_sync(~0u, ok) & 0xffffu;
+#pragma unroll
+    for (int j = 0; j < kInsn; ++j) {
+      const int r = kPieces <= 32 ? j * kRows : j / 2, c = kPieces <= 32 ? 0 : 32 * (j & 1);
+      const long long o = __shfl_sync(~0u, off, r0 + r);
+      if (c0 + c < pieces) copy16(to + r * S::pitch + 16 * c, base + o + 16 * (c0 + c), (mask >> (r0 + r)) & 1);
     }
     return mask;
   };
 
-  // queries: 16-bit as B fragments in registers, fp32 as high and low parts in
-  // shared memory (heads beyond the group are zeros)
-  unsigned qf[S::wide ? 1 : NT][S::wide ? 1 : HD / 16][2];
-  unsigned char* q_sm = sm + (S::ring > S::join ? S::ring : S::join);
-  const T* qrow = (const T*)a.q + row * a.ldq + (long long)head0 * a.hd;
+  // The ring holds units K0 V0 K1 V1 ..., kAhead of them in flight; unit u lies
+  // in slot u % units, and the copy of unit u + kAhead goes into the slot that
+  // unit u - 1 has just left.
+  constexpr int kAhead = S::units - 1, kSteps = kAhead / 2;
+  static_assert(kAhead % 2 == 0, "K and V of a step are issued alike");
+  unsigned masks[kSteps + 1];
   int pg = page_at(0);
 #pragma unroll
-  for (int i = 0; i < S::stages - 1; ++i) {
+  for (int i = 0; i < kSteps; ++i) {
     const int next = page_at(i + 1);
-    masks[i] = issue(i, pg, i);
+    masks[i] = issue(kbase, i, pg, 2 * i);
+    copies_done();
+    issue(vbase, i, pg, 2 * i + 1);
     copies_done();
     pg = next;
   }
-  masks[S::stages - 1] = 0;
+
+  // queries: 16-bit as B fragments in registers, fp32 as high and low parts in
+  // shared memory (heads beyond the group are zeros)
+  unsigned qf[S::wide ? 1 : NT][S::wide ? 1 : HD / 16][2];
+  unsigned char* q_sm = sm + S::base;
+  const T* qrow = (const T*)a.q + row * a.ldq + (long long)head0 * a.hd;
   if constexpr (S::wide) {
     for (int i = threadIdx.x; i < S::heads * HD; i += S::warps * 32) {
       const int h = i / HD, d = i % HD;
       const float x = h < heads && d < a.hd ? ((const float*)qrow)[h * a.hd + d] : 0.f;
       unsigned hi, lo;
       split_tf32(x, hi, lo);
-      *reinterpret_cast<unsigned*>(q_sm + h * S::k_pitch + 4 * d) = hi;
-      *reinterpret_cast<unsigned*>(q_sm + (S::heads + h) * S::k_pitch + 4 * d) = lo;
+      *reinterpret_cast<unsigned*>(q_sm + h * S::q_pitch + 4 * d) = hi;
+      *reinterpret_cast<unsigned*>(q_sm + (S::heads + h) * S::q_pitch + 4 * d) = lo;
     }
     __syncthreads();
   } else {
@@ -278,14 +357,15 @@ paged_attn_kernel(const AttnArgs a) {
           qf[n][ks][b] = h < heads && d < a.hd ? *reinterpret_cast<const unsigned*>(qrow + h * a.hd + d) : 0u;
         }
   }
-  __syncwarp();
 
+  // Per head (columns 2 q4 + j of tile n): the reference m, which starts below
+  // every score, the sum l of this lane's weights, the accumulators.
   float o[HD / 16][NT][4];
   float m_ref[NT][2], l[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) { m_ref[n][j] = -INFINITY; l[n][j] = 0.f; }
+    for (int j = 0; j < 2; ++j) { m_ref[n][j] = -FLT_MAX; l[n][j] = 0.f; }
 #pragma unroll
     for (int mt = 0; mt < HD / 16; ++mt)
 #pragma unroll
@@ -295,36 +375,31 @@ paged_attn_kernel(const AttnArgs a) {
   // largest still round to something
   constexpr float kLift = std::is_same<T, __half>::value ? 6.0f : 0.0f;
 
-  int st = 0, fill = S::stages - 1;
+  int slot = 0;
+  auto before = [&](int s) { return s == 0 ? S::units - 1 : s - 1; };
+  auto after = [&](int s) { return s + 1 == S::units ? 0 : s + 1; };
   for (int i = 0; i < mine; ++i) {
-    wait_copies<S::stages - 2>();
+    wait_copies<kAhead - 1>();
     __syncwarp();
-    // the stage emptied by the step before is filled while this one is used
-    {
-      const int next = page_at(i + S::stages);
-      masks[S::stages - 1] = issue(i + S::stages - 1, pg, fill);
-      copies_done();
-      pg = next;
-    }
-    const unsigned mask = masks[0];
-    const unsigned char* kst = ring + st * S::stage;
-    const unsigned char* vst = kst + kStep * S::k_pitch;
+    const int next = page_at(i + kSteps + 1);
+    masks[kSteps] = issue(kbase, i + kSteps, pg, before(slot));
+    copies_done();
+    const unsigned char* kst = ring + slot * S::unit;
+    slot = after(slot);
 
-    // S^T: positions g, g+8 (rows) x heads 2 q4, 2 q4 + 1 (columns)
+    // S^T: positions g, g + 8 (rows) x heads 2 q4, 2 q4 + 1 (columns)
     float s[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
     if constexpr (S::wide) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[0][j] = 0.f;
 #pragma unroll 4
       for (int kk = 0; kk < HD / 16; ++kk) {
         // 16 columns: lane q4 holds columns 4 q4 .. 4 q4 + 3, the first two
         // as one k-step of 8, the other two as the next
-        const float4 x = *reinterpret_cast<const float4*>(kst + g * S::k_pitch + 64 * kk + 16 * q4);
-        const float4 y = *reinterpret_cast<const float4*>(kst + (g + 8) * S::k_pitch + 64 * kk + 16 * q4);
-        const uint4 bh = *reinterpret_cast<const uint4*>(q_sm + g * S::k_pitch + 64 * kk + 16 * q4);
-        const uint4 bl = *reinterpret_cast<const uint4*>(q_sm + (S::heads + g) * S::k_pitch + 64 * kk + 16 * q4);
+        const float4 x = *reinterpret_cast<const float4*>(kst + swap01(g) * S::pitch + 64 * kk + 16 * q4);
+        const float4 y = *reinterpret_cast<const float4*>(kst + (swap01(g) + 8) * S::pitch + 64 * kk + 16 * q4);
+        const uint4 bh = *reinterpret_cast<const uint4*>(q_sm + g * S::q_pitch + 64 * kk + 16 * q4);
+        const uint4 bl = *reinterpret_cast<const uint4*>(q_sm + (S::heads + g) * S::q_pitch + 64 * kk + 16 * q4);
         unsigned ah[4], al[4], ch[4], cl[4];
         split_tf32(x.x, ah[0], al[0]); split_tf32(y.x, ah[1], al[1]);
         split_tf32(x.y, ah[2], al[2]); split_tf32(y.y, ah[3], al[3]);
@@ -341,25 +416,47 @@ paged_attn_kernel(const AttnArgs a) {
         for (int j = 0; j < 4; ++j) s[0][j] += c[j] + d[j];
       }
     } else {
-      const unsigned ka = smem_u32(kst) + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::k_pitch + (lane >> 4) * 16;
+      // two accumulators a tile: half the chain of dependent products
+      const unsigned ka = smem_u32(kst) + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::pitch + (lane >> 4) * 16;
+      float e[NT][4];
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        unsigned af[4];
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = e[n][j] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ks += 2) {
+        unsigned af[4], bf[4];
         ldsm4(af, ka + ks * 32);
+        ldsm4(bf, ka + ks * 32 + 32);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16<T>(s[n], af, qf[n][ks][0], qf[n][ks][1]);
+        for (int n = 0; n < NT; ++n) {
+          mma16<T>(s[n], af, qf[n][ks][0], qf[n][ks][1]);
+          mma16<T>(e[n], bf, qf[n][ks + 1][0], qf[n][ks + 1][1]);
+        }
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] += e[n][j];
     }
-    const bool v0 = (mask >> g) & 1, v1 = (mask >> (g + 8)) & 1;
+    if (masks[0] != 0xffffu) {
+      const int gt = S::wide ? swap01(g) : g;
+      const bool v0 = (masks[0] >> gt) & 1, v1 = (masks[0] >> (gt + 8)) & 1;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = ((j < 2) ? v0 : v1) ? s[n][j] * a.scale_log2 : -INFINITY;
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] *= a.scale_log2;
+    }
     bool raise = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[n][j] = ((j < 2) ? v0 : v1) ? s[n][j] * a.scale_log2 : -INFINITY;
-        raise |= s[n][j] > m_ref[n][j & 1] + (kLift + kRaise);
-      }
-    }
+      for (int j = 0; j < 2; ++j) raise |= fmaxf(s[n][j], s[n][j + 2]) - m_ref[n][j] > kLift + kRaise;
     if (__any_sync(~0u, raise)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -369,8 +466,7 @@ paged_attn_kernel(const AttnArgs a) {
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
-          const float to = fmaxf(m_ref[n][j], mx - kLift);
-          const float f = m_ref[n][j] == to ? 1.0f : exp2f(m_ref[n][j] - to);   // -inf - -inf is not taken
+          const float to = fmaxf(m_ref[n][j], mx - kLift), f = ex2(m_ref[n][j] - to);
           m_ref[n][j] = to;
           l[n][j] *= f;
 #pragma unroll
@@ -380,21 +476,25 @@ paged_attn_kernel(const AttnArgs a) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float m = m_ref[n][j & 1] == -INFINITY ? 0.f : m_ref[n][j & 1];
-        s[n][j] = exp2f(s[n][j] - m);
-      }
+      for (int j = 0; j < 4; ++j) s[n][j] = ex2(s[n][j] - m_ref[n][j & 1]);
       l[n][0] += s[n][0] + s[n][2];
       l[n][1] += s[n][1] + s[n][3];
     }
 
+    wait_copies<kAhead - 1>();
+    __syncwarp();
+    issue(vbase, i + kSteps, pg, before(slot));
+    copies_done();
+    pg = next;
+    const unsigned char* vst = ring + slot * S::unit;
+    slot = after(slot);
     // O^T += V^T P^T
     if constexpr (S::wide) {
       // P^T fragments: position q4 (+4, +8, +12) of head g
       unsigned ph[4], pl[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int src = ((j & 1) * 4 + q4) * 4 + (g >> 1);
+        const int src = swap01((j & 1) * 4 + q4) * 4 + (g >> 1);
         const float e0 = __shfl_sync(~0u, s[0][(j >> 1) * 2], src);
         const float e1 = __shfl_sync(~0u, s[0][(j >> 1) * 2 + 1], src);
         split_tf32((g & 1) ? e1 : e0, ph[j], pl[j]);
@@ -406,7 +506,7 @@ paged_attn_kernel(const AttnArgs a) {
         float4 x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          x[j] = *reinterpret_cast<const float4*>(vst + (q4 + 4 * j) * S::v_pitch + 128 * b + 16 * g);
+          x[j] = *reinterpret_cast<const float4*>(vst + (q4 + 4 * j) * S::pitch + 128 * b + 16 * g);
         float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
         unsigned ah[2][4], al[2][4], ch[2][4], cl[2][4];
 #pragma unroll
@@ -442,7 +542,7 @@ paged_attn_kernel(const AttnArgs a) {
           ph[n][j] = turn8x8(hi);
           pl[n][j] = turn8x8(lo);
         }
-      const unsigned va = smem_u32(vst) + ((lane & 7) + (lane >> 4) * 8) * S::v_pitch + ((lane >> 3) & 1) * 16;
+      const unsigned va = smem_u32(vst) + ((lane & 7) + (lane >> 4) * 8) * S::pitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
       for (int mt = 0; mt < HD / 16; ++mt) {
         unsigned af[4];
@@ -455,9 +555,7 @@ paged_attn_kernel(const AttnArgs a) {
       }
     }
 #pragma unroll
-    for (int j = 0; j + 1 < S::stages; ++j) masks[j] = masks[j + 1];
-    st = st + 1 == S::stages ? 0 : st + 1;
-    fill = fill + 1 == S::stages ? 0 : fill + 1;
+    for (int j = 0; j < kSteps; ++j) masks[j] = masks[j + 1];
   }
 
   // ---- join the warps ----
@@ -466,6 +564,7 @@ paged_attn_kernel(const AttnArgs a) {
   float* jo = reinterpret_cast<float*>(sm);                       // [warp][head][HD]
   float* jm = jo + S::warps * S::heads * HD;                      // [warp][head]
   float* jl = jm + S::warps * S::heads;
+  float *co = jl + S::warps * S::heads, *cm = co + S::heads * HD;   // clustered: the CTA's result
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -489,66 +588,214 @@ paged_attn_kernel(const AttnArgs a) {
   for (int i = threadIdx.x; i < heads * (HD / 4); i += S::warps * 32) {
     const int h = i / (HD / 4), d = i % (HD / 4) * 4;
     if (d >= a.hd) continue;
-    float m = -INFINITY;
+    float m = -FLT_MAX;
 #pragma unroll
     for (int w = 0; w < S::warps; ++w) m = fmaxf(m, jm[w * S::heads + h]);
-    const float m0 = m == -INFINITY ? 0.f : m;
     float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < S::warps; ++w) {
-      const float f = exp2f(jm[w * S::heads + h] - m0);
+      const float f = ex2(jm[w * S::heads + h] - m);
       const float4 x = *reinterpret_cast<const float4*>(jo + (w * S::heads + h) * HD + d);
       sum = fmaf(f, jl[w * S::heads + h], sum);
       acc[0] = fmaf(f, x.x, acc[0]); acc[1] = fmaf(f, x.y, acc[1]);
       acc[2] = fmaf(f, x.z, acc[2]); acc[3] = fmaf(f, x.w, acc[3]);
     }
     const long long rh = (long long)row * a.n_q + head0 + h;
-    if (rn.n == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] *= inv;
-      using V = at::Vec4<T>;
-      *reinterpret_cast<typename V::raw*>((T*)a.out + row * a.ldo + (long long)(head0 + h) * a.hd + d) = V::put(acc);
-      if (a.lse && d == 0) a.lse[rh] = (m + log2f(sum)) * 0.6931471805599453f;
+    if (parts == 1) {
+      store_out<T>(a, row, head0 + h, d, acc, sum, m);
+      if (d == 0 && a.mode != kClustered && a.parts > 1) a.part_ml[rh * a.parts] = make_float2(m, -0.f);
+    } else if (a.mode == kClustered) {
+      *reinterpret_cast<float4*>(co + h * HD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (d == 0) { cm[2 * h] = m; cm[2 * h + 1] = sum; }
     } else {
       *reinterpret_cast<float4*>(a.part_o + (rh * a.parts + part) * a.hd + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (d == 0) a.part_ml[rh * a.parts + part] = make_float2(m, sum);
+      // the sign of l marks a row's last run (the sum itself is not negative)
+      const unsigned mark = part == parts - 1 ? 1u << 31 : 0u;
+      if (d == 0)
+        a.part_ml[rh * a.parts + part] = make_float2(m, __uint_as_float((__float_as_uint(sum) & 0x7fffffffu) | mark));
     }
+  }
+  if (a.mode != kClustered || parts == 1) return;
+  // ---- join the cluster's CTAs, each of them a share of the elements ----
+  cluster_sync();
+  for (int i = part * S::warps * 32 + threadIdx.x; i < heads * (HD / 4); i += parts * S::warps * 32) {
+    const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+    if (d >= a.hd) continue;
+    float2 ml[kCluster];
+    float4 x[kCluster];
+    float m = -FLT_MAX;
+#pragma unroll
+    for (int p = 0; p < kCluster; ++p) {
+      ml[p] = p < parts ? remote2(cm + 2 * h, p) : make_float2(-FLT_MAX, 0.f);
+      x[p] = p < parts ? remote4(co + h * HD + d, p) : make_float4(0.f, 0.f, 0.f, 0.f);
+      m = fmaxf(m, ml[p].x);
+    }
+    float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < kCluster; ++p) {
+      const float f = ex2(ml[p].x - m);
+      sum = fmaf(f, ml[p].y, sum);
+      acc[0] = fmaf(f, x[p].x, acc[0]); acc[1] = fmaf(f, x[p].y, acc[1]);
+      acc[2] = fmaf(f, x[p].z, acc[2]); acc[3] = fmaf(f, x[p].w, acc[3]);
+    }
+    store_out<T>(a, row, head0 + h, d, acc, sum, m);
+  }
+}
+
+// A row without positions: zeros.
+template <typename T>
+__device__ __forceinline__ void clear_heads(const AttnArgs& a, int row, int head0, int heads) {
+  for (int i = threadIdx.x; i < heads * a.hd; i += blockDim.x)
+    store1<T>(a.out, row * a.ldo + (long long)head0 * a.hd + i, 0.f);
+  if (a.lse)
+    for (int h = threadIdx.x; h < heads; h += blockDim.x) a.lse[(long long)row * a.n_q + head0 + h] = -INFINITY;
+}
+
+// How the work is split, a "item" being a row's key-value head and tile:
+//   kDealt      The pieces of all items, one after another, are cut into as
+//               many equal stretches as there are CTAs, which is what the GPU
+//               holds at a time. A stretch may end one item and begin the next,
+//               so a ragged batch leaves no CTA waiting for the longest row.
+//               Every warp works the cut out for itself from the rows' lengths.
+//               A second launch joins the items' runs.
+//   kClustered  An item is a cluster's: each CTA takes an equal run, and they
+//               join through distributed shared memory. One launch, for short
+//               contexts, where the second one would be most of the time.
+//   kRuns       A CTA takes one run of 8 pieces at least (or, with room for one
+//               part only, the item): for rows too many to be dealt.
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(Shape<T, HD, NT>::warps * 32, Shape<T, HD, NT>::ctas)
+paged_attn_kernel(const AttnArgs a) {
+  using S = Shape<T, HD, NT>;
+  extern __shared__ __align__(16) unsigned char sm[];
+  pdl_wait();
+  pdl_launch();
+  const int lane = threadIdx.x & 31, kt = a.n_kv * a.tiles;
+
+  int row, len, u;                  // the current row, its positions and pieces
+  int run_part = 0;
+  int base, w, w1, stretch;         // where its items' pieces begin; this CTA's pieces; pieces a CTA
+  if (a.mode == kDealt) {
+    for (row = blockIdx.x; row < a.rows; row += gridDim.x)
+      if (length_of(a, row) == 0) clear_heads<T>(a, row, 0, a.n_q);
+    const int per = (a.rows + 31) / 32, r0 = min(lane * per, a.rows), r1 = min(r0 + per, a.rows);
+    int sum = 0, most = 0, last_len = 0;
+    for (int r = r0; r < r1; ++r) {
+      last_len = length_of(a, r);
+      const int n = pieces_of(last_len);
+      sum += n;
+      most = max(most, n);
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const int total = __shfl_sync(~0u, upto, 31) * kt;
+    most = __reduce_max_sync(~0u, most);
+    // long enough that no item is cut into more than a.parts runs: u pieces
+    // meet at most (u - 2) / stretch + 2 stretches
+    stretch = max(max(1, (total - 1) / (int)gridDim.x + 1), (most + a.parts - 3) / (a.parts - 1));
+    if ((long long)blockIdx.x * stretch >= total) return;
+    w = blockIdx.x * stretch;
+    w1 = total - w < stretch ? total : w + stretch;
+    const int owner = __ffs(__ballot_sync(~0u, upto * kt > w)) - 1;
+    row = owner * per;
+    base = __shfl_sync(~0u, upto - sum, owner) * kt;
+    len = per == 1 ? __shfl_sync(~0u, last_len, owner) : length_of(a, row);
+    u = pieces_of(len);
+  } else {
+    run_part = blockIdx.x % a.parts;
+    const int item = blockIdx.x / a.parts, i = item % kt;
+    row = item / kt;
+    len = length_of(a, row);
+    if (len < 0) return;
+    if (len == 0) {
+      const int tile = i % a.tiles;
+      if (run_part == 0)
+        clear_heads<T>(a, row, i / a.tiles * a.group + tile * S::heads, min(S::heads, a.group - tile * S::heads));
+      return;
+    }
+    u = pieces_of(len);
+    stretch = (u - 1) / a.parts + 1;
+    if (a.mode == kRuns && a.parts > 1) stretch = max(8, stretch);
+    w = min(run_part * stretch, u);
+    w1 = min(w + stretch, u);
+    // a cluster's CTA without a run of its own still takes part in the join
+    if (w >= w1 && a.mode != kClustered) return;
+    const int parts = a.mode == kClustered ? a.parts : (u - 1) / stretch + 1;
+    attend<T, HD, NT>(a, sm, row, i / a.tiles, i % a.tiles, min(len, w * kPiece), min(len, w1 * kPiece), run_part, parts);
+    if (a.mode == kClustered && parts > 1) cluster_sync();     // the others may still be reading here
+    return;
+  }
+  for (;;) {
+    while (base + u * kt <= w) {
+      base += u * kt;
+      len = length_of(a, ++row);
+      u = pieces_of(len);
+    }
+    const int item = (w - base) / u, off = (w - base) - item * u, n = min(u - off, w1 - w), start = base + item * u;
+    const int first = start / stretch, last = (start + u - 1) / stretch;
+    attend<T, HD, NT>(a, sm, row, item / a.tiles, item % a.tiles, off * kPiece, min(len, (off + n) * kPiece),
+                      blockIdx.x - first, last - first + 1);
+    w += n;
+    if (w >= w1) return;
+    __syncthreads();                // the ring is free again
   }
 }
 
 // Joins the runs of a row: a block per (row, query head), the runs dealt to
-// its 8 warps, each lane four (or eight) elements of the head.
+// its 8 warps, each lane four (or eight) elements of the head. Its time is the
+// latency of its loads, so the first 4 runs of every warp are loaded beside
+// the runs' maxima and sums, before it is known how many runs there are (what
+// lies behind them in the workspace is not used).
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const AttnArgs a) {
   __shared__ float sw[kMaxParts], red[kJoinWarps][256], total;
   const int row = blockIdx.x / a.n_q, h = blockIdx.x % a.n_q;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int len = length_of(a, row);             // written before the launch that this one follows
+  const long long base = ((long long)row * a.n_q + h) * a.parts;
   // every block waits, those without work too: what follows this launch in
   // the stream relies on the first kernel's results being there
   pdl_wait();
-  const int seq = a.row_seq ? a.row_seq[row] : row;
-  if (seq < 0 || seq >= a.n_seq) return;
-  const Runs rn = runs_of(a.row_pos[row], a.capacity, a.parts);
-  if (rn.n <= 1) return;
-  const long long base = ((long long)row * a.n_q + h) * a.parts;
+  pdl_launch();
+  if (len <= 0) return;
+  float2 ml[kMaxParts / 32];
+#pragma unroll
+  for (int j = 0; j < kMaxParts / 32; ++j) {
+    const int p = j * 32 + lane;
+    ml[j] = p < a.parts ? a.part_ml[base + p] : make_float2(0.f, 0.f);
+  }
+  float4 x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int p = warp + j * kJoinWarps;
+    x[j] = p < a.parts && 4 * lane < a.hd ? *reinterpret_cast<const float4*>(a.part_o + (base + p) * a.hd + 4 * lane)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  int n = 0;                                     // runs: the last one is marked
+#pragma unroll
+  for (int j = 0; j < kMaxParts / 32; ++j) {
+    const unsigned marks = __ballot_sync(~0u, __float_as_uint(ml[j].y) >> 31);
+    if (n == 0 && marks) n = j * 32 + __ffs(marks);
+  }
+  if (n <= 1) return;                            // its only run has written the result
+  float m = -FLT_MAX;
+#pragma unroll
+  for (int j = 0; j < kMaxParts / 32; ++j) {
+    ml[j] = j * 32 + lane < n ? make_float2(ml[j].x, fabsf(ml[j].y)) : make_float2(-FLT_MAX, 0.f);
+    m = fmaxf(m, ml[j].x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
   if (warp == 0) {
-    float2 ml[kMaxParts / 32];
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kMaxParts / 32; ++j) {
-      const int p = j * 32 + lane;
-      ml[j] = p < rn.n ? a.part_ml[base + p] : make_float2(-INFINITY, 0.f);
-      m = fmaxf(m, ml[j].x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    const float m0 = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < kMaxParts / 32; ++j) {
-      const float f = exp2f(ml[j].x - m0);
+      const float f = ex2(ml[j].x - m);
       sw[j * 32 + lane] = f;
       sum = fmaf(f, ml[j].y, sum);
     }
@@ -562,21 +809,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attn_join_kernel(const 
   __syncthreads();
   for (int d = 4 * lane; d < a.hd; d += 128) {
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = warp; p < rn.n; p += kJoinWarps) {
+    auto add = [&](int p, const float4& v) {
       const float f = sw[p];
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + (base + p) * a.hd + d);
-      acc[0] = fmaf(f, x.x, acc[0]); acc[1] = fmaf(f, x.y, acc[1]);
-      acc[2] = fmaf(f, x.z, acc[2]); acc[3] = fmaf(f, x.w, acc[3]);
+      acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]);
+      acc[2] = fmaf(f, v.z, acc[2]); acc[3] = fmaf(f, v.w, acc[3]);
+    };
+    int p = warp;
+    if (d < 128) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j, p += kJoinWarps)
+        if (p < n) add(p, x[j]);
     }
+#pragma unroll 6
+    for (; p < n; p += kJoinWarps) add(p, *reinterpret_cast<const float4*>(a.part_o + (base + p) * a.hd + d));
     *reinterpret_cast<float4*>(&red[warp][d]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < a.hd; d += kJoinWarps * 32) {
-    float x = 0.f;
+    float y = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) x += red[w][d];
-    store1<T>(a.out, row * a.ldo + (long long)h * a.hd + d, total == 0.f ? 0.f : x / total);
+    for (int w = 0; w < kJoinWarps; ++w) y += red[w][d];
+    store1<T>(a.out, row * a.ldo + (long long)h * a.hd + d, total == 0.f ? 0.f : y / total);
   }
 }
 
@@ -586,22 +839,33 @@ int head_tile(int dtype, int hd, int group) {
   return dtype != MOE_DTYPE_F32 && hd <= 128 && group > 8 ? 16 : 8;
 }
 
-// How many runs a row may be split into. Rows and key-value heads alone that
-// fill the GPU's two CTAs per SM need no split for parallelism, but a ragged
-// batch does for balance: runs of 512 positions.
-int parts_of(int rows, int n_kv, int tiles, int max_kv) {
-  const long long items = (long long)rows * n_kv * tiles;
-  long long parts = (296 + items - 1) / items;
-  if (items >= 4) parts = 296 / items;
-  const long long even = (max_kv - 1) / 512 + 1, most = (max_kv - 1) / kMinRun + 1;
-  if (rows > 1 && parts < even) parts = even;
-  if (parts > most) parts = most;
-  if (parts > kMaxParts) parts = kMaxParts;
-  return parts < 1 ? 1 : (int)parts;
+// The split of a call, from what the host knows of it, and the parts that a
+// row's head may have. Short contexts: clusters that together are about four
+// CTAs per SM, of one CTA where the items alone are that many.
+struct Split { int mode, parts; };
+Split split_of(long long items, int rows, int max_kv) {
+  const int pieces = (max_kv - 1) / kPiece + 1;
+  if (pieces <= kShort) {
+    int n = 1;
+    while (n < kCluster && n < pieces && items * n < 592) n *= 2;
+    return {n > 1 ? kClustered : kRuns, n};
+  }
+  return {rows <= kDealtRows ? kDealt : kRuns, pieces < kMaxParts ? pieces : kMaxParts};
+}
+
+int sm_count(int device) {
+  static std::atomic<int> count[64];
+  if (device < 0 || device >= 64) return 148;
+  int n = count[device].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) n = 148;
+    count[device].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 template <typename T, int HD, int NT>
-cudaError_t launch_attn(const AttnArgs& a, int device, cudaStream_t st) {
+cudaError_t launch_attn(AttnArgs a, int max_kv, int device, cudaStream_t st) {
   using S = Shape<T, HD, NT>;
   static std::atomic<unsigned long long> ready{0};       // devices whose limit is raised
   const unsigned long long bit = 1ull << (device & 63);
@@ -611,21 +875,44 @@ cudaError_t launch_attn(const AttnArgs& a, int device, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (device < 64) ready.fetch_or(bit, std::memory_order_release);
   }
-  const unsigned grid = (unsigned)((long long)a.rows * a.n_kv * a.tiles * a.parts);
-  paged_attn_kernel<T, HD, NT><<<grid, S::warps * 32, S::smem, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.parts == 1) return e;
+  const long long items = (long long)a.rows * a.n_kv * a.tiles, sms = sm_count(device);
+  long long grid = items * a.parts;
+  if (a.mode == kDealt) {
+    // what the GPU holds at a time; where an item's parts are too few for
+    // that, the largest whole number of CTAs per SM that they allow; and no
+    // more CTAs than pieces
+    const long long room = sms * S::ctas, most = items * (a.parts - 1), all = items * ((max_kv - 1) / kPiece + 1);
+    grid = most >= room ? room : most >= sms ? most / sms * sms : most;
+    if (grid > all) grid = all;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(S::warps * 32); cfg.dynamicSmemBytes = S::smem; cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.mode == kClustered) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = a.parts; at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, HD, NT>, a);
+  if (e != cudaSuccess || a.mode == kClustered || a.parts == 1) return e;
   return launch_pdl(paged_attn_join_kernel<T>, dim3((unsigned)a.rows * (unsigned)a.n_q), dim3(kJoinWarps * 32), 0, st, a);
 }
 
 template <typename T>
-cudaError_t launch_type(const AttnArgs& a, int tile, int device, cudaStream_t st) {
+cudaError_t launch_type(const AttnArgs& a, int tile, int max_kv, int device, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    if (tile == 16) return a.hd <= 64 ? launch_attn<T, 64, 2>(a, device, st) : launch_attn<T, 128, 2>(a, device, st);
+    if (tile == 16) return a.hd <= 64 ? launch_attn<T, 64, 2>(a, max_kv, device, st) : launch_attn<T, 128, 2>(a, max_kv, device, st);
   }
-  if (a.hd <= 64) return launch_attn<T, 64, 1>(a, device, st);
-  if (a.hd <= 128) return launch_attn<T, 128, 1>(a, device, st);
-  return launch_attn<T, 256, 1>(a, device, st);
+  if (a.hd <= 64) return launch_attn<T, 64, 1>(a, max_kv, device, st);
+  if (a.hd <= 128) return launch_attn<T, 128, 1>(a, max_kv, device, st);
+  return launch_attn<T, 256, 1>(a, max_kv, device, st);
 }
 
 }  // namespace
@@ -637,9 +924,10 @@ extern "C" size_t moe_paged_attention_workspace(int rows, int n_q, const MoeKvCa
   if (at::check_cache(cache, "moe_paged_attention_workspace")) return 0;
   if (rows < 1 || n_q < 1 || n_q % cache->n_kv || max_kv < 1) return 0;
   const int group = n_q / cache->n_kv, ht = head_tile(cache->dtype, cache->head_dim, group);
-  const int parts = parts_of(rows, cache->n_kv, (group + ht - 1) / ht, max_kv);
-  if (parts == 1) return 0;
-  return (size_t)rows * n_q * parts * (sizeof(float2) + sizeof(float) * cache->head_dim) + 16;
+  const long long items = (long long)rows * cache->n_kv * ((group + ht - 1) / ht);
+  const Split sp = split_of(items, rows, max_kv);
+  if (sp.parts == 1 || sp.mode == kClustered) return 0;
+  return (size_t)rows * n_q * sp.parts * (sizeof(float2) + sizeof(float) * cache->head_dim) + 16;
 }
 
 extern "C" int moe_paged_attention_dev(const void* q, long long ldq, const MoeKvCache* cache, const int* block_table,
@@ -665,8 +953,14 @@ extern "C" int moe_paged_attention_dev(const void* q, long long ldq, const MoeKv
   const int group = n_q / cache->n_kv, ht = head_tile(cache->dtype, hd, group);
   AttnArgs a{};
   a.tiles = (group + ht - 1) / ht;
-  a.parts = parts_of(rows, cache->n_kv, a.tiles, max_kv);
-  if ((long long)rows * cache->n_kv * a.tiles * a.parts > INT32_MAX || (long long)rows * n_q > INT32_MAX)
+  const long long items = (long long)rows * cache->n_kv * a.tiles;
+  const Split sp = split_of(items, rows, max_kv);
+  a.parts = sp.parts;
+  a.mode = sp.mode;
+  // pieces are numbered in 32 bits where they are dealt out
+  const long long pieces = (long long)max_pages * cache->page_size / kPiece + 1;
+  if (a.mode == kDealt && items * pieces > INT32_MAX) a.mode = kRuns;
+  if (items * a.parts > INT32_MAX || (long long)rows * n_q > INT32_MAX)
     return at::fail(MOE_ERR_UNSUPPORTED, "%s: too many rows and heads for one launch", who);
   const size_t need = moe_paged_attention_workspace(rows, n_q, cache, max_kv);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
@@ -687,9 +981,8 @@ extern "C" int moe_paged_attention_dev(const void* q, long long ldq, const MoeKv
   a.part_ml = (float2*)((char*)workspace + ((size_t)rows * n_q * a.parts * hd * sizeof(float) + 15) / 16 * 16);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
-  if (cache->dtype == MOE_DTYPE_BF16) e = launch_type<__nv_bfloat16>(a, ht, on.device(), st);
-  else if (cache->dtype == MOE_DTYPE_F16) e = launch_type<__half>(a, ht, on.device(), st);
-  else e = launch_type<float>(a, ht, on.device(), st);
-  if (e != cudaSuccess) { cudaGetLastError(); return at::fail(MOE_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e)); }
-  return MOE_OK;
+  if (cache->dtype == MOE_DTYPE_BF16) e = launch_type<__nv_bfloat16>(a, ht, max_kv, on.device(), st);
+  else if (cache->dtype == MOE_DTYPE_F16) e = launch_type<__half>(a, ht, max_kv, on.device(), st);
+  else e = launch_type<float>(a, ht, max_kv, on.device(), st);
+  return at::launched(e, who);
 }

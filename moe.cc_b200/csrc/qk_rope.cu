@@ -35,6 +35,8 @@ constexpr int kThreads = 128;
 
 template <typename TI, typename TO, int LPH>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs a) {
+  pdl_wait();
+  pdl_launch();
   using VI = at::Vec4<TI>;
   using VO = at::Vec4<TO>;
   const int row = blockIdx.x, g = threadIdx.x / LPH, l = threadIdx.x % LPH;
@@ -108,18 +110,18 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs a
 }
 
 template <typename TI, typename TO>
-void launch_rope(const RopeArgs& a, int rows, cudaStream_t st) {
+cudaError_t launch_rope(const RopeArgs& a, int rows, cudaStream_t st) {
   const int heads = a.n_q + 2 * a.n_kv;
   auto go = [&](auto kernel, int lph) {
     // few rows: one head per lane group, so that the row spreads over blocks;
     // many rows: a block keeps its row's table entries for all heads
     const int per = kThreads / lph, full = (heads + per - 1) / per;
     const int y = rows >= 1184 ? 1 : full;
-    kernel<<<dim3(rows, y), kThreads, 0, st>>>(a);
+    return launch_pdl(kernel, dim3(rows, y), dim3(kThreads), 0, st, a);
   };
-  if (a.hd <= 64) go(qk_norm_rope_kernel<TI, TO, 8>, 8);
-  else if (a.hd <= 128) go(qk_norm_rope_kernel<TI, TO, 16>, 16);
-  else go(qk_norm_rope_kernel<TI, TO, 32>, 32);
+  if (a.hd <= 64) return go(qk_norm_rope_kernel<TI, TO, 8>, 8);
+  if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 16>, 16);
+  return go(qk_norm_rope_kernel<TI, TO, 32>, 32);
 }
 
 // whether the row-strided ranges [p, p + ((rows-1) ld + n) es) of two
@@ -186,11 +188,11 @@ extern "C" int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k,
   a.n_slots = cache->n_pages * cache->page_size; a.page_size = cache->page_size; a.eps = eps;
   a.page = at::FastDiv((unsigned)cache->page_size);
   cudaStream_t st = (cudaStream_t)stream;
-  if (es == 2) {
-    if (dtype == MOE_DTYPE_BF16) launch_rope<__nv_bfloat16, __nv_bfloat16>(a, rows, st);
-    else launch_rope<__half, __half>(a, rows, st);
-  } else if (cache->dtype == MOE_DTYPE_F32) launch_rope<float, float>(a, rows, st);
-  else if (cache->dtype == MOE_DTYPE_BF16) launch_rope<float, __nv_bfloat16>(a, rows, st);
-  else launch_rope<float, __half>(a, rows, st);
-  return at::launched(who);
+  cudaError_t e;
+  if (dtype == MOE_DTYPE_BF16) e = launch_rope<__nv_bfloat16, __nv_bfloat16>(a, rows, st);
+  else if (dtype == MOE_DTYPE_F16) e = launch_rope<__half, __half>(a, rows, st);
+  else if (cache->dtype == MOE_DTYPE_F32) e = launch_rope<float, float>(a, rows, st);
+  else if (cache->dtype == MOE_DTYPE_BF16) e = launch_rope<float, __nv_bfloat16>(a, rows, st);
+  else e = launch_rope<float, __half>(a, rows, st);
+  return at::launched(e, who);
 }

@@ -407,40 +407,55 @@ def moe_ffn_ep(layer, x_norm2, x_inout, stream=None):
 # torch CUDA tensors; `stream` as in the calls above. A tensor of the wrong type,
 # place or layout is refused here, before its pointer is handed on.
 
-_ELEM = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+class _Types:
+    """torch's types, looked up when the first tensor comes (this module does
+    not import torch)."""
+    elem = None
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.i32, cls.f32 = torch.int32, torch.float32
+        cls.elem = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
 def _elem(t, what):
-    d = _ELEM.get(str(t.dtype))
+    if _Types.elem is None:
+        _Types.load()
+    d = _Types.elem.get(t.dtype)
     if d is None:
         raise MoeError(MOE_ERR_INVALID, f"{what}: float32, float16 or bfloat16 is wanted, got {t.dtype}")
     return d
 
 
-def _dev(t, kind, shape, what, device):
-    """Pointer of a contiguous device tensor of the given type and shape (None: any length); None passes through."""
+def _dev(t, dtype, shape, what, device):
+    """Pointer of a contiguous tensor of the given type and shape on CUDA
+    device number `device`; None passes through."""
     if t is None:
         return None
-    if str(t.dtype) != kind or not t.is_contiguous() or t.device != device or t.dim() != len(shape) or any(
-            n is not None and m != n for m, n in zip(t.shape, shape)):
-        raise MoeError(MOE_ERR_INVALID, f"{what}: a contiguous {kind} tensor of shape {shape} on {device} is wanted, "
-                                        f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise MoeError(MOE_ERR_INVALID, f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{device} is "
+                                        f"wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _rows(t, what, heads, hd, device):
     """(pointer, row stride) of [rows][heads][head_dim] whose rows may lie apart."""
-    if t.dim() != 3 or t.device != device or t.shape[2] != hd or (heads is not None and t.shape[1] != heads) or (
-            t.numel() and ((hd > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != hd))):
-        raise MoeError(MOE_ERR_INVALID, f"{what}: [rows][heads][{hd}] on {device} with contiguous rows is wanted, "
-                                        f"got {tuple(t.shape)}, strides {t.stride()} on {t.device}")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1] * hd)
+    shape, st = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != hd or shape[1] != heads or t.get_device() != device or (
+            (st[2] != 1 and hd > 1 or st[1] != hd and heads > 1) and t.numel()):
+        raise MoeError(MOE_ERR_INVALID, f"{what}: [rows][{heads}][{hd}] on cuda:{device} with contiguous rows is wanted, "
+                                        f"got {tuple(shape)}, strides {st} on {t.device}")
+    return t.data_ptr(), (st[0] if shape[0] > 1 else heads * hd)
 
 
 def _cuda_device(t, what):
+    """The number of the CUDA device that holds t."""
     if not t.is_cuda:
         raise MoeError(MOE_ERR_INVALID, f"{what}: a CUDA tensor is wanted")
-    return t.device
+    if _Types.elem is None:
+        _Types.load()
+    return t.get_device()
 
 
 def kv_cache(k, v):
@@ -461,14 +476,15 @@ def kv_cache(k, v):
 def kv_plan(past_len, new_len, page_size, n_pages, free_pages, block_table, row_seq, row_pos, row_slot, kv_len=None,
             free_head=None, free_head_out=None, status=None, stream=None):
     """moe_kv_plan_dev: int32 tensors; past_len may be None (nothing held yet)."""
-    n, mp = block_table.shape
-    dev, cap, i32 = _cuda_device(block_table, "kv_plan"), row_seq.shape[0], "torch.int32"
+    dev, i32 = _cuda_device(block_table, "kv_plan"), _Types.i32
+    (n, mp), rows, free = block_table.shape, row_seq.shape, free_pages.shape
+    seqs = (n,)
     check(lib().moe_kv_plan_dev(
-        _dev(past_len, i32, (n,), "past_len", dev), _dev(new_len, i32, (n,), "new_len", dev), n, page_size, n_pages,
-        _dev(free_pages, i32, (None,), "free_pages", dev), free_pages.shape[0], _dev(free_head, i32, (1,), "free_head", dev),
-        _dev(block_table, i32, (n, mp), "block_table", dev), mp, _dev(kv_len, i32, (n,), "kv_len", dev),
-        _dev(row_seq, i32, (cap,), "row_seq", dev), _dev(row_pos, i32, (cap,), "row_pos", dev),
-        _dev(row_slot, i32, (cap,), "row_slot", dev), cap, _dev(free_head_out, i32, (1,), "free_head_out", dev),
+        _dev(past_len, i32, seqs, "past_len", dev), _dev(new_len, i32, seqs, "new_len", dev), n, page_size, n_pages,
+        _dev(free_pages, i32, (free.numel(),), "free_pages", dev), free[0], _dev(free_head, i32, (1,), "free_head", dev),
+        _dev(block_table, i32, (n, mp), "block_table", dev), mp, _dev(kv_len, i32, seqs, "kv_len", dev),
+        _dev(row_seq, i32, (rows.numel(),), "row_seq", dev), _dev(row_pos, i32, rows, "row_pos", dev),
+        _dev(row_slot, i32, rows, "row_slot", dev), rows[0], _dev(free_head_out, i32, (1,), "free_head_out", dev),
         _dev(status, i32, (3,), "status", dev), _stream(stream)))
 
 
@@ -479,7 +495,7 @@ def qk_norm_rope(q, k, v, k_cache, v_cache, row_pos, row_slot, q_out, rope=None,
     [positions][rot_dim] fp32, the cosines then the sines; row_slot None:
     queries only (k, v are then not read and may be None)."""
     c = kv_cache(k_cache, v_cache)
-    hd, dev, i32, f32 = c.head_dim, _cuda_device(k_cache, "qk_norm_rope"), "torch.int32", "torch.float32"
+    hd, dev, i32, f32 = c.head_dim, _cuda_device(k_cache, "qk_norm_rope"), _Types.i32, _Types.f32
     x = q if q is not None else k
     rows, dt = x.shape[0], _elem(x, "q")
     qp = op = kp = vp = None
@@ -488,14 +504,15 @@ def qk_norm_rope(q, k, v, k_cache, v_cache, row_pos, row_slot, q_out, rope=None,
         n_q = q.shape[1]
         qp, ldq = _rows(q, "q", n_q, hd, dev)
         op, ldo = _rows(q_out, "q_out", n_q, hd, dev)
-        if q_out.dtype != k_cache.dtype or q_out.shape[0] != rows:
+        if q_out.dtype is not k_cache.dtype or q_out.shape[0] != rows:
             raise MoeError(MOE_ERR_INVALID, "q_out: the rows of q in the cache's type are wanted")
     if row_slot is not None:
-        kp, ldk = _rows(k, "k", c.n_kv, hd, dev)
-        vp, ldv = _rows(v, "v", c.n_kv, hd, dev)
-        if k.dtype != x.dtype or v.dtype != x.dtype or k.shape[0] != rows or v.shape[0] != rows:
+        n_kv = c.n_kv
+        kp, ldk = _rows(k, "k", n_kv, hd, dev)
+        vp, ldv = _rows(v, "v", n_kv, hd, dev)
+        if k.dtype is not x.dtype or v.dtype is not x.dtype or k.shape[0] != rows or v.shape[0] != rows:
             raise MoeError(MOE_ERR_INVALID, "q, k and v: one type and one number of rows")
-    rot, n_rope = (rope.shape[1], rope.shape[0]) if rope is not None else (0, 0)
+    n_rope, rot = rope.shape if rope is not None else (0, 0)
     check(lib().moe_qk_norm_rope_dev(
         qp, ldq, kp, ldk, vp, ldv, dt, rows, n_q, _dev(q_norm, f32, (hd,), "q_norm", dev),
         _dev(k_norm, f32, (hd,), "k_norm", dev), eps, _dev(rope, f32, (n_rope, rot), "rope", dev), rot, n_rope,
@@ -513,40 +530,40 @@ def paged_attention(q, k_cache, v_cache, block_table, row_pos, out, workspace, m
     """moe_paged_attention_dev. q, out [rows][n_q][head_dim]; workspace: a
     contiguous tensor of any type (None where none is needed)."""
     c = kv_cache(k_cache, v_cache)
-    dev, i32 = _cuda_device(k_cache, "paged_attention"), "torch.int32"
-    rows, n_q = q.shape[0], q.shape[1]
-    qp, ldq = _rows(q, "q", n_q, c.head_dim, dev)
-    op, ldo = _rows(out, "out", n_q, c.head_dim, dev)
-    if q.dtype != k_cache.dtype or out.dtype != k_cache.dtype or out.shape[0] != rows:
+    dev, i32, hd, dt = _cuda_device(k_cache, "paged_attention"), _Types.i32, c.head_dim, k_cache.dtype
+    rows, n_q = q.shape[:2]
+    qp, ldq = _rows(q, "q", n_q, hd, dev)
+    op, ldo = _rows(out, "out", n_q, hd, dev)
+    if q.dtype is not dt or out.dtype is not dt or out.shape[0] != rows:
         raise MoeError(MOE_ERR_INVALID, "q and out: the same rows in the cache's type are wanted")
     n_seq, mp = block_table.shape
     wp, wn = None, 0
     if workspace is not None:
-        if not workspace.is_contiguous() or workspace.device != dev:
-            raise MoeError(MOE_ERR_INVALID, f"workspace: a contiguous tensor on {dev} is wanted")
-        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if not workspace.is_contiguous() or workspace.get_device() != dev:
+            raise MoeError(MOE_ERR_INVALID, f"workspace: a contiguous tensor on cuda:{dev} is wanted")
+        wp, wn = workspace.data_ptr(), workspace.nbytes
     check(lib().moe_paged_attention_dev(
         qp, ldq, C.byref(c), _dev(block_table, i32, (n_seq, mp), "block_table", dev), n_seq, mp,
         _dev(row_seq, i32, (rows,), "row_seq", dev), _dev(row_pos, i32, (rows,), "row_pos", dev), rows, n_q, max_kv, scale,
-        op, ldo, _dev(lse, "torch.float32", (rows, n_q), "lse", dev), wp, wn, _stream(stream)))
+        op, ldo, _dev(lse, _Types.f32, (rows, n_q), "lse", dev), wp, wn, _stream(stream)))
 
 
 def route(logits, topk_idx, topk_p, bias=None, score="softmax", groups=1, keep_groups=1, group_top=1, renorm=True,
           scale=1.0, stream=None):
     """moe_route_dev: topk_idx (int32) and topk_p (fp32) [rows][top_k] of
     logits [rows][E] (rows may lie apart)."""
-    dev = _cuda_device(logits, "route")
-    T, E = logits.shape
-    if T and E > 1 and logits.stride(1) != 1:
+    dev, dt = _cuda_device(logits, "route"), _elem(logits, "logits")
+    (T, E), st = logits.shape, logits.stride()
+    if st[1] != 1 and T and E > 1:
         raise MoeError(MOE_ERR_INVALID, "logits: the experts must be contiguous")
-    if score not in ROUTE_SCORES:
+    kind = ROUTE_SCORES.get(score)
+    if kind is None:
         raise MoeError(MOE_ERR_INVALID, f"score: one of {sorted(ROUTE_SCORES)} is wanted")
-    k = topk_idx.shape[1]
+    shape = (T, topk_idx.shape[1])
     check(lib().moe_route_dev(
-        logits.data_ptr(), logits.stride(0) if T > 1 else E, _elem(logits, "logits"), T, E,
-        _dev(bias, "torch.float32", (E,), "bias", dev), ROUTE_SCORES[score], groups, keep_groups, group_top, k,
-        int(bool(renorm)), scale, _dev(topk_idx, "torch.int32", (T, k), "topk_idx", dev),
-        _dev(topk_p, "torch.float32", (T, k), "topk_p", dev), _stream(stream)))
+        logits.data_ptr(), st[0] if T > 1 else E, dt, T, E, _dev(bias, _Types.f32, (E,), "bias", dev), kind, groups,
+        keep_groups, group_top, shape[1], 1 if renorm else 0, scale, _dev(topk_idx, _Types.i32, shape, "topk_idx", dev),
+        _dev(topk_p, _Types.f32, shape, "topk_p", dev), _stream(stream)))
 
 
 def profile(enable):

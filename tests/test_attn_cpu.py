@@ -35,7 +35,7 @@ def rope(c=None, **over):
 
 def attn(c=None, **over):
     c = c or cache()
-    d = dict(q=P, ldq=256, cache=C.byref(c), table=P, n_seq=4, max_pages=8, seq=None, pos=P, rows=4, n_q=4, max_kv=128,
+    d = dict(q=P, ldq=256, cache=C.byref(c), table=P, n_seq=4, max_pages=8, seq=None, pos=P, rows=4, n_q=4, max_kv=4096,
              scale=0.1, out=P, ldo=256, lse=None, ws=P, n=1 << 30)
     d.update(over)
     return mc.lib().moe_paged_attention_dev(*d.values(), None)
@@ -101,14 +101,15 @@ def test_attention_refuses(over, want):
 
 
 def test_attention_workspace_size():
-    """No workspace where a row is one run; otherwise a row of head_dim + 2 floats per query head and run, at most 128 runs."""
+    """None for contexts up to 2048 positions (one launch); above, a row of
+    head_dim + 2 floats per query head and 64 positions, at most 128."""
     ws = mc.lib().moe_paged_attention_workspace
-    assert ws(4, 4, C.byref(cache()), 64) == 0
-    assert ws(0, 4, C.byref(cache()), 64) == 0 and ws(4, 3, C.byref(cache()), 64) == 0 and ws(4, 4, C.byref(cache()), 0) == 0
-    for rows, n_q, max_kv in ((1, 2, 100), (1, 32, 1 << 20), (33, 8, 8192), (1, 2, 2**31 - 1)):
+    for rows, n_q, max_kv in ((1, 2, 1), (4, 4, 64), (1, 32, 2048), (600, 4, 1000), (0, 4, 4096), (4, 3, 4096), (4, 4, 0)):
+        assert ws(rows, n_q, C.byref(cache()), max_kv) == 0
+    for rows, n_q, max_kv in ((1, 2, 2049), (1, 32, 1 << 20), (33, 8, 8192), (600, 4, 5000), (1, 2, 2**31 - 1)):
         n = ws(rows, n_q, C.byref(cache()), max_kv)
         one = rows * n_q * (64 + 2) * 4
-        assert 2 * one <= n <= min(128, -(-max_kv // 64)) * one + 16
+        assert n == min(128, -(-max_kv // 64)) * one + 16
 
 
 @pytest.mark.parametrize("over,want", [

@@ -149,35 +149,24 @@ template <> __device__ __forceinline__ void store1<__half>(void* p, long long i,
 
 // Shapes of one instantiation. HD: head_dim rounded up to 64, 128 or 256 (the
 // columns between are zeros in shared memory); NT: 8-head column tiles.
-#ifndef PA_W16
-#define PA_W16 4
-#endif
-#ifndef PA_U16
-#define PA_U16 3
-#endif
-#ifndef PA_C16
-#define PA_C16 2
-#endif
-#ifndef PA_W32
-#define PA_W32 (HD == 64 ? 8 : 4)
-#endif
-#ifndef PA_C32
-#define PA_C32 (HD == 128 ? 2 : 1)
-#endif
-#ifndef PA_U32
-#define PA_U32 3
-#endif
 template <typename T, int HD, int NT>
 struct Shape {
   static constexpr bool wide = sizeof(T) == 4;
-  // A row's pitch keeps the fragment loads free of bank conflicts: 16-bit rows
-  // an odd number of 16-byte pieces (ldmatrix), fp32 rows 8 words past a
-  // multiple of 32 (16-byte loads of 2 rows two apart, or of 4 rows 8 words each).
-  static constexpr int pitch = wide ? HD * 4 + 32 : HD * 2 + 16;
+  // The rows lie so that the fragment loads meet no bank conflicts and every
+  // 32-byte sector of a row stays one aligned 32-byte block: with rows 16 bytes
+  // off (a pitch of an odd number of pieces) each of their sectors crossed the
+  // crossbar twice. 16-bit rows: piece c of row r at c ^ (r & 7) (ldmatrix).
+  // fp32 rows: 8 words past a multiple of 32 (16-byte loads of 2 rows two
+  // apart, or of 4 rows 8 words each).
+  static constexpr int pitch = wide ? HD * 4 + 32 : HD * 2;
   static constexpr int unit = kStep * pitch;       // the K or the V rows of a step
-  static constexpr int warps = wide ? (HD == 256 ? 4 : PA_W32) : HD == 256 ? 8 : NT == 2 ? 4 : PA_W16;
-  static constexpr int units = wide ? (HD == 64 ? 5 : PA_U32) : HD == 256 ? 3 : NT == 2 || HD == 64 ? 5 : PA_U16;
-  static constexpr int ctas = wide ? PA_C32 : HD == 256 ? 1 : NT == 2 ? 2 : PA_C16;
+  // Warps, ring units a warp and CTAs an SM: 8 to 12 warps, 100 to 150 KB of
+  // ring. 16-bit rows of 128, 32 rows of up to 8192 positions / one row of
+  // 131072: 3 CTAs of 4 warps 59.4 / 49.1 us, 2 of 4 60.8 / 49.0, 4 of 4 60.2 /
+  // 48.7, 1 of 8 64.5 / 50.0, 5 units in 2 CTAs of 4 60.7 / 49.5.
+  static constexpr int warps = wide && HD == 64 || !wide && HD == 256 ? 8 : 4;
+  static constexpr int units = HD == 64 || NT == 2 ? 5 : 3;
+  static constexpr int ctas = HD == 256 || wide && HD == 64 ? 1 : wide || NT == 2 ? 2 : 3;
   static constexpr int heads = 8 * NT;
   static constexpr int q_pitch = HD * 4 + 64;      // fp32: Q's high and low parts, rows 16 words past
   static constexpr int q_bytes = wide ? 2 * heads * q_pitch : 0;
@@ -258,8 +247,10 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
   // columns from head_dim to HD are zeros throughout: no copy touches them
   if (pieces < kPieces) {
     const int pad = kPieces - pieces;
-    for (int i = lane; i < S::units * kStep * pad; i += 32)
-      *reinterpret_cast<uint4*>(ring + i / pad * S::pitch + 16 * (pieces + i % pad)) = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < S::units * kStep * pad; i += 32) {
+      const int r = i / pad, c = pieces + i % pad;
+      *reinterpret_cast<uint4*>(ring + r * S::pitch + 16 * (S::wide ? c : c ^ (r & 7))) = make_uint4(0, 0, 0, 0);
+    }
   }
 
   // Page of step i (of position `lane & 15` of it, where a step may span
@@ -274,11 +265,15 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
   constexpr int kRows = kPieces <= 32 ? 32 / kPieces : 1;      // rows one instruction of the warp covers
   constexpr int kInsn = kStep * kPieces / 32;
   const int r0 = kPieces <= 32 ? lane / kPieces : 0, c0 = kPieces <= 32 ? lane % kPieces : lane;
+  const int d0 = r0 * S::pitch + 16 * (S::wide ? c0 : c0 ^ r0);
+  // where this lane's piece of row r0 + r goes (16-bit: kRows divides 8 and
+  // r0 < kRows, so (r0 + r) & 7 is r0 ^ (r & 7))
+  auto place = [&](int r, int c) { return S::wide ? d0 + r * S::pitch + 16 * c : (d0 ^ (16 * (r & 7))) + r * S::pitch; };
   auto issue = [&](const char* base, int i, int pg, int slot) -> unsigned {
     if (i >= mine) return 0u;
     const int t = t0 + (i * S::warps + warp) * kStep;
     const bool ok = pg >= 0 && pg < a.n_pages;
-    const unsigned to = smem_u32(ring + slot * S::unit) + r0 * S::pitch + 16 * c0;
+    const unsigned to = smem_u32(ring + slot * S::unit);
     if (whole) {
       const int n = ok ? min(kStep, t1 - t) : 0;
       const int in = t - (int)a.page.div((unsigned)t) * a.page_size;
@@ -288,7 +283,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
 #pragma unroll
           for (int j = 0; j < kInsn; ++j) {
             const int r = kPieces <= 32 ? j * kRows : j / 2, c = kPieces <= 32 ? 0 : 32 * (j & 1);
-            copy16(to + r * S::pitch + 16 * c, src + 16 * c);
+            copy16(to + place(r, c), src + 16 * c);
             if (kPieces <= 32 || (j & 1)) src += kRows * row_bytes;
           }
         }
@@ -297,7 +292,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
 #pragma unroll 1
       for (int j = 0; j < kInsn; ++j) {
         const int r = kPieces <= 32 ? j * kRows : j / 2, c = kPieces <= 32 ? 0 : 32 * (j & 1);
-        if (c0 + c < pieces) copy16(to + r * S::pitch + 16 * c, src + r * row_bytes + 16 * c, r0 + r < n);
+        if (c0 + c < pieces) copy16(to + place(r, c), src + r * row_bytes + 16 * c, r0 + r < n);
       }
       return (1u << n) - 1u;
     }
@@ -309,7 +304,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
     for (int j = 0; j < kInsn; ++j) {
       const int r = kPieces <= 32 ? j * kRows : j / 2, c = kPieces <= 32 ? 0 : 32 * (j & 1);
       const long long o = __shfl_sync(~0u, off, r0 + r);
-      if (c0 + c < pieces) copy16(to + r * S::pitch + 16 * c, base + o + 16 * (c0 + c), (mask >> (r0 + r)) & 1);
+      if (c0 + c < pieces) copy16(to + place(r, c), base + o + 16 * (c0 + c), (mask >> (r0 + r)) & 1);
     }
     return mask;
   };
@@ -417,7 +412,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
       }
     } else {
       // two accumulators a tile: half the chain of dependent products
-      const unsigned ka = smem_u32(kst) + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::pitch + (lane >> 4) * 16;
+      const unsigned ka = smem_u32(kst) + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::pitch;
+      const unsigned kx = 16 * ((lane >> 4) ^ (lane & 7));
       float e[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -426,8 +422,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks += 2) {
         unsigned af[4], bf[4];
-        ldsm4(af, ka + ks * 32);
-        ldsm4(bf, ka + ks * 32 + 32);
+        ldsm4(af, ka + (kx ^ (ks * 32)));
+        ldsm4(bf, ka + (kx ^ (ks * 32 + 32)));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma16<T>(s[n], af, qf[n][ks][0], qf[n][ks][1]);
@@ -542,11 +538,12 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
           ph[n][j] = turn8x8(hi);
           pl[n][j] = turn8x8(lo);
         }
-      const unsigned va = smem_u32(vst) + ((lane & 7) + (lane >> 4) * 8) * S::pitch + ((lane >> 3) & 1) * 16;
+      const unsigned va = smem_u32(vst) + ((lane & 7) + (lane >> 4) * 8) * S::pitch;
+      const unsigned vx = 16 * (((lane >> 3) & 1) ^ (lane & 7));
 #pragma unroll
       for (int mt = 0; mt < HD / 16; ++mt) {
         unsigned af[4];
-        ldsm4t(af, va + mt * 32);
+        ldsm4t(af, va + (vx ^ (mt * 32)));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma16<T>(o[mt][n], af, ph[n][0], ph[n][1]);

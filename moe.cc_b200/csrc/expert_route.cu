@@ -9,19 +9,25 @@
 //   top k by c, ties to the lower index; p = s, divided by the sum of the
 //   chosen s if wanted, times a factor
 //
-// Scores, choices and sums are held in 64 bits: the choice is an ordering, and
-// in fp32 two different sigmoid scores near 1 (or scores plus a bias) round to
-// the same number often enough to change which expert is chosen. An exp in
-// double costs little here: E of them per token, at B200's 64 double-precision
-// lanes per SM. Without a bias or groups the order of the scores is the order
-// of the logits, and then only the chosen experts' scores are computed (and
-// the softmax's sum, where the weights are not renormalised).
+// The choice is an ordering, and it is the order of the exact scores that is
+// wanted: in fp32 two different sigmoid scores near 1 (or scores plus a bias)
+// round to the same number often enough to change which expert is chosen.
+// Without a bias or groups the order of the scores is the order of the logits,
+// exactly, and no score is needed for it. Otherwise a token is first ranked by
+// fp32 scores, whose error is bounded (`margin`); where two neighbours of the
+// ranking, the last chosen and the first left out included, or the groups on
+// either side of the cut, are closer than that, the token is ranked again by
+// scores in 64 bits. About 1 token in 100 is. The weights are fp32 softmax or
+// sigmoid values of the chosen.
 //
 // One warp routes one token: expert j * 32 + lane in lane `lane`. A round of
-// the selection takes the largest 64-bit key by two 32-bit warp reductions and
-// the lowest index that has it by a third, so k rounds are k times about 40
-// instructions. Small calls are bound by the launch and those rounds' latency.
+// the selection takes the largest key by a warp reduction, then the lowest
+// index that has it by another; 16-bit logits carry the index in the key's
+// other half and need one. Issue slots are the bound: a token costs a few
+// hundred instructions a warp, its logits a few hundred bytes.
 #include "attn.cuh"
+
+#include <type_traits>
 
 namespace moe {
 namespace {
@@ -35,15 +41,22 @@ struct RouteArgs {
   float* p;
   long long ld;
   int rows, E, softmax, groups, keep, group_top, topk, renorm, lanes_per_group, group_size;
-  double factor;
+  float factor;
 };
 
-// order-preserving 64-bit key of a choice; 0 is below every number's key
+// order-preserving keys; 0 is below every number's key, and -0 and 0 are one
 __device__ __forceinline__ unsigned long long key_of(double c) {
-  const long long b = __double_as_longlong(c + 0.0);      // -0 and 0 are one value
+  const long long b = __double_as_longlong(c + 0.0);
   return (unsigned long long)b ^ (b < 0 ? ~0ull : 1ull << 63);
 }
-__device__ __forceinline__ double warp_sum64(double v) {
+__device__ __forceinline__ unsigned key_of(float c) {
+  const int b = __float_as_int(c + 0.0f);
+  return (unsigned)b ^ (b < 0 ? ~0u : 1u << 31);
+}
+__device__ __forceinline__ float value_of(unsigned key) {
+  return __uint_as_float(key >> 31 ? key ^ (1u << 31) : ~key);
+}
+template <typename F> __device__ __forceinline__ F warp_sum_of(F v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   return v;
@@ -54,142 +67,247 @@ template <> __device__ __forceinline__ float logit<float>(const void* x, long lo
 template <> __device__ __forceinline__ float logit<__nv_bfloat16>(const void* x, long long i) { return __bfloat162float(((const __nv_bfloat16*)x)[i]); }
 template <> __device__ __forceinline__ float logit<__half>(const void* x, long long i) { return __half2float(((const __half*)x)[i]); }
 
-// exp(x - top) with x = top = +inf counted as 1
-__device__ __forceinline__ double weight_of(float x, float top) { return x == top ? 1.0 : exp((double)x - (double)top); }
-__device__ __forceinline__ double sigmoid64(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
+// exp(x - top) with x = top = +inf counted as 1, and the sigmoid, in the type of the ranking
+__device__ __forceinline__ float soft(float x, float top) { return x == top ? 1.0f : expf(x - top); }
+__device__ __forceinline__ float sigm(float x) { return 1.0f / (1.0f + expf(-x)); }
+__device__ __forceinline__ double soft64(float x, float top) { return x == top ? 1.0 : exp((double)x - (double)top); }
+__device__ __forceinline__ double sigm64(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
+
+// Scores plus bias of a lane's experts, in F; -inf for an expert that may not
+// be chosen (a NaN or -inf logit or bias).
+template <typename F, int EPL>
+__device__ __forceinline__ void choices(const RouteArgs& a, const float (&x)[EPL], float top, F (&c)[EPL]) {
+  const int lane = threadIdx.x & 31;
+  F sum = 0;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    if constexpr (sizeof(F) == 8) c[j] = a.softmax ? soft64(x[j], top) : sigm64(x[j]);
+    else c[j] = a.softmax ? soft(x[j], top) : sigm(x[j]);
+    if (!(x[j] > -INFINITY)) c[j] = 0;
+    sum += c[j];
+  }
+  if (a.softmax) {
+    sum = warp_sum_of(sum);
+    if constexpr (sizeof(F) == 8) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) c[j] = c[j] / sum;
+    } else {
+      const float inv = 1.0f / sum;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) c[j] *= inv;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    if (a.bias && j * 32 + lane < a.E) c[j] += (F)a.bias[j * 32 + lane];
+    if (!(x[j] > -INFINITY && c[j] > -INFINITY)) c[j] = -INFINITY;
+  }
+}
+
+// How far apart two fp32 choices must be for the exact ones to be ordered
+// alike. In units of 2^-24: a sigmoid errs by 4 (expf by 2 ulp, damped by
+// e^-x s < 1, sum and quotient); a softmax score relatively by |z| (its rounded
+// argument z = x - max; |z| s < 0.4), 4 (expf), 2 (quotient and product) and by
+// its sum: up to 37 roundings and the mean of |z|, below ln 1024 + 1; together
+// less than 2^6. A sum with the bias adds its own rounding. Two of them: 2^-17.
+__device__ __forceinline__ float margin(float u, float v) { return 0x1p-17f * (1.0f + fabsf(u) + fabsf(v)); }
+
+// Takes the experts outside the `keep` best groups out of c. cut[0], cut[1]:
+// the least sum that stays and the largest that does not.
+template <typename F, int EPL>
+__device__ __forceinline__ void keep_groups(const RouteArgs& a, F* mine, F (&c)[EPL], F (&cut)[2]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) mine[j * 32 + lane] = c[j];
+  __syncwarp();
+  // lanes_per_group lanes look through a group and merge their best two
+  const int lpg = a.lanes_per_group, grp = lane / lpg;
+  F b0 = -INFINITY, b1 = -INFINITY;
+  if (grp < a.groups)
+    for (int i = lane % lpg; i < a.group_size; i += lpg) {
+      const F v = mine[grp * a.group_size + i];
+      b1 = max(b1, min(b0, v));
+      b0 = max(b0, v);
+    }
+  for (int o = 1; o < lpg; o <<= 1) {
+    const F o0 = __shfl_xor_sync(~0u, b0, o), o1 = __shfl_xor_sync(~0u, b1, o);
+    b1 = max(min(b0, o0), max(b1, o1));
+    b0 = max(b0, o0);
+  }
+  const F gs = b0 + (a.group_top == 2 && b1 > -INFINITY ? b1 : (F)0);
+  // a group stays if fewer than `keep` groups come before it
+  int before = 0;
+  for (int h = 0; h < a.groups; ++h) {
+    const F v = __shfl_sync(~0u, gs, h * lpg);
+    before += v > gs || (v == gs && h < grp);
+  }
+  const bool head = grp < a.groups && lane % lpg == 0;
+  const unsigned stays = __ballot_sync(~0u, head && before < a.keep);
+  cut[0] = __shfl_sync(~0u, gs, __ffs(__ballot_sync(~0u, head && before == a.keep - 1)) - 1);
+  cut[1] = __shfl_sync(~0u, gs, __ffs(__ballot_sync(~0u, head && before == a.keep)) - 1);
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int e = j * 32 + lane, ge = e / a.group_size;
+    if (e < a.E && !((stays >> (ge * lpg)) & 1)) c[j] = -INFINITY;
+  }
+}
+
+// One round: the largest of the warp's keys, the lowest expert that has it
+// (which then leaves), or -1.
+template <int EPL>
+__device__ __forceinline__ int take(unsigned (&key)[EPL], unsigned& top) {
+  const int lane = threadIdx.x & 31;
+  unsigned best = key[0];
+  int at = 0;
+#pragma unroll
+  for (int j = 1; j < EPL; ++j)
+    if (key[j] > best) { best = key[j]; at = j; }
+  top = __reduce_max_sync(~0u, best);
+  if (top == 0u) return -1;
+  const unsigned mine = at * 32 + lane, e = __reduce_min_sync(~0u, best == top ? mine : ~0u);
+#pragma unroll
+  for (int j = 0; j < EPL; ++j)
+    if (j * 32 + lane == e) key[j] = 0u;
+  return (int)e;
+}
+template <int EPL>
+__device__ __forceinline__ int take(unsigned long long (&key)[EPL]) {
+  const int lane = threadIdx.x & 31;
+  unsigned long long best = key[0];
+  int at = 0;
+#pragma unroll
+  for (int j = 1; j < EPL; ++j)
+    if (key[j] > best) { best = key[j]; at = j; }
+  const unsigned hi = (unsigned)(best >> 32), top_hi = __reduce_max_sync(~0u, hi);
+  const unsigned lo = hi == top_hi ? (unsigned)best : 0u, top_lo = __reduce_max_sync(~0u, lo);
+  if ((top_hi | top_lo) == 0u) return -1;
+  const bool cand = hi == top_hi && lo == top_lo;
+  const unsigned mine = at * 32 + lane, e = __reduce_min_sync(~0u, cand ? mine : ~0u);
+#pragma unroll
+  for (int j = 0; j < EPL; ++j)
+    if (j * 32 + lane == e) key[j] = 0ull;
+  return (int)e;
+}
+
+// The token's choice ranked in 64 bits; lane r returns the r-th.
+template <int EPL>
+__device__ __noinline__ int choose64(const RouteArgs& a, const float (&x)[EPL], float top, double* mine) {
+  double c[EPL];
+  unsigned long long key[EPL];
+  choices<double, EPL>(a, x, top, c);
+  if (a.groups > 1) {
+    double cut[2];
+    keep_groups<double, EPL>(a, mine, c, cut);
+  }
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) key[j] = c[j] > -INFINITY ? key_of(c[j]) : 0ull;
+  int chosen = -1;
+  for (int r = 0; r < a.topk; ++r) {
+    const int e = take<EPL>(key);
+    if (e < 0) break;
+    if ((threadIdx.x & 31) == r) chosen = e;
+  }
+  return chosen;
+}
 
 // EPL experts a lane; SCORED: the choice needs every score (bias or groups)
 template <typename T, int EPL, bool SCORED>
 __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteArgs a) {
+  extern __shared__ double choice_sm[];                    // groups: [kWarps][EPL * 32]
   pdl_wait();
   pdl_launch();
-  extern __shared__ double choice_sm[];                    // groups: [kWarps][EPL * 32]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = (long long)blockIdx.x * kWarps + warp;
   if (t >= a.rows) return;
   float x[EPL];
-  float top = -INFINITY;
+  unsigned key[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = j * 32 + lane;
     x[j] = e < a.E ? logit<T>(a.x, t * a.ld + e) : -INFINITY;
     if (!(x[j] > -INFINITY)) x[j] = -INFINITY;            // NaN: never chosen, as -inf
-    top = fmaxf(top, x[j]);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-
-  double total = 1.0;
-  unsigned long long key[EPL];
+  float top = -INFINITY;
+  int chosen = -1;                                         // lane r: the r-th choice
   if constexpr (SCORED) {
-    double c[EPL];
-    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
+    const unsigned tk = __reduce_max_sync(~0u, key_of(top));
+    top = value_of(tk);
+    float c[EPL], cut[2] = {INFINITY, -INFINITY};
+    choices<float, EPL>(a, x, top, c);
+    if (a.groups > 1) keep_groups<float, EPL>(a, (float*)(choice_sm + warp * (EPL * 32)), c, cut);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) key[j] = c[j] > -INFINITY ? key_of(c[j]) : 0u;
+    float last = INFINITY;
+    bool close = cut[0] - cut[1] < 2 * margin(cut[0], cut[1]);
+    for (int r = 0; r <= a.topk; ++r) {                    // one more than is taken: the first left out
+      unsigned k;
+      const int e = take<EPL>(key, k);
+      if (e < 0) break;
+      const float v = value_of(k);
+      close |= !(last - v >= margin(last, v));
+      last = v;
+      if (lane == r && r < a.topk) chosen = e;
+    }
+    if (close) chosen = choose64<EPL>(a, x, top, choice_sm + warp * (EPL * 32));
+  } else if constexpr (sizeof(T) == 2) {
+    // the logit's 16 bits above, the index from the top down below them
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      const bool in = x[j] > -INFINITY;
-      c[j] = !in ? 0.0 : a.softmax ? weight_of(x[j], top) : sigmoid64(x[j]);
-      sum += c[j];
+      const unsigned e = j * 32 + lane;
+      unsigned b;
+      if constexpr (std::is_same<T, __half>::value) b = __half_as_ushort(__float2half_rn(x[j] + 0.0f));
+      else b = __float_as_uint(x[j] + 0.0f) >> 16;
+      b = (b ^ (b >> 15 ? 0xffffu : 0x8000u)) & 0xffffu;
+      key[j] = x[j] > -INFINITY ? b << 16 | (0xffffu - e) : 0u;
     }
-    if (a.softmax) total = warp_sum64(sum);
+    for (int r = 0; r < a.topk; ++r) {
+      unsigned best = key[0];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      if (a.softmax) c[j] = c[j] / total;
-      if (a.bias && j * 32 + lane < a.E) c[j] += (double)a.bias[j * 32 + lane];
-      const bool in = x[j] > -INFINITY && c[j] > -INFINITY;    // a NaN or -inf bias hides its expert
-      if (!in) c[j] = -INFINITY;
-      key[j] = in ? key_of(c[j]) : 0ull;
-    }
-    if (a.groups > 1) {
-      double* mine = choice_sm + warp * (EPL * 32);
+      for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
+      best = __reduce_max_sync(~0u, best);
+      if (best == 0u) break;
+      if (lane == r) chosen = 0xffff - (int)(best & 0xffffu);
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) mine[j * 32 + lane] = c[j];
-      __syncwarp();
-      // lanes_per_group lanes look through a group and merge their best two
-      const int lpg = a.lanes_per_group, grp = lane / lpg;
-      double b0 = -INFINITY, b1 = -INFINITY;
-      if (grp < a.groups)
-        for (int i = lane % lpg; i < a.group_size; i += lpg) {
-          const double v = mine[grp * a.group_size + i];
-          if (v > b0) { b1 = b0; b0 = v; } else if (v > b1) b1 = v;
-        }
-      for (int o = 1; o < lpg; o <<= 1) {
-        const double o0 = __shfl_xor_sync(~0u, b0, o), o1 = __shfl_xor_sync(~0u, b1, o);
-        const double lo = b0 > o0 ? o0 : b0;
-        b1 = fmax(lo, fmax(b1, o1));
-        b0 = fmax(b0, o0);
-      }
-      const double gs = b0 + (a.group_top == 2 && b1 > -INFINITY ? b1 : 0.0);
-      // a group stays if fewer than `keep` groups come before it
-      int before = 0;
-      for (int h = 0; h < a.groups; ++h) {
-        const double v = __shfl_sync(~0u, gs, h * lpg);
-        before += v > gs || (v == gs && h < grp);
-      }
-      const unsigned stays = __ballot_sync(~0u, grp < a.groups && before < a.keep && lane % lpg == 0);
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        const int e = j * 32 + lane, ge = e / a.group_size;
-        if (e >= a.E || !((stays >> (ge * lpg)) & 1)) key[j] = 0ull;
-      }
+      for (int j = 0; j < EPL; ++j) key[j] = key[j] == best ? 0u : key[j];
     }
   } else {
-    if (a.softmax && !a.renorm) {
-      double sum = 0.0;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) sum += x[j] > -INFINITY ? weight_of(x[j], top) : 0.0;
-      total = warp_sum64(sum);
-    }
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const int b = __float_as_int(x[j] + 0.0f);
-      const unsigned k = (unsigned)b ^ (b < 0 ? ~0u : 1u << 31);
-      key[j] = x[j] > -INFINITY ? k : 0u;
+    for (int j = 0; j < EPL; ++j) key[j] = x[j] > -INFINITY ? key_of(x[j]) : 0u;
+    for (int r = 0; r < a.topk; ++r) {
+      unsigned k;
+      const int e = take<EPL>(key, k);
+      if (e < 0) break;
+      if (lane == r) chosen = e;
     }
   }
 
-  // k rounds; lane r keeps the r-th choice
-  int chosen = -1;
-  for (int r = 0; r < a.topk; ++r) {
-    unsigned long long best = key[0];
-    int at = 0;
-#pragma unroll
-    for (int j = 1; j < EPL; ++j)
-      if (key[j] > best) { best = key[j]; at = j; }
-    bool cand = true;
-    unsigned any;
-    if constexpr (SCORED) {
-      const unsigned hi = (unsigned)(best >> 32), top_hi = __reduce_max_sync(~0u, hi);
-      cand = hi == top_hi;
-      any = top_hi;
-      const unsigned lo = cand ? (unsigned)best : 0u, top_lo = __reduce_max_sync(~0u, lo);
-      cand = cand && lo == top_lo;
-      any |= top_lo;
-    } else {
-      any = __reduce_max_sync(~0u, (unsigned)best);
-      cand = (unsigned)best == any;
-    }
-    if (any == 0u) break;                                  // no expert is left
-    const unsigned e = __reduce_min_sync(~0u, cand ? (unsigned)(at * 32 + lane) : ~0u);
-    if (lane == r) chosen = (int)e;
-    if (cand && (unsigned)(at * 32 + lane) == e) {
-#pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (j == at) key[j] = 0ull;
-    }
-  }
-
-  double s = 0.0;
-  if (chosen >= 0) {
-    const float xe = logit<T>(a.x, t * a.ld + chosen);
-    s = a.softmax ? weight_of(xe, top) / total : sigmoid64(xe);
-  }
+  const float xe = chosen >= 0 ? logit<T>(a.x, t * a.ld + chosen) : 0.f;
+  float s;
   if (a.renorm) {
-    const double sum = warp_sum64(s);
-    s = sum > 0.0 ? s / sum : 0.0;
+    // only ratios matter: from the largest chosen logit, so that they survive
+    // where the scores themselves would underflow (far below 0 the sigmoid is
+    // the exponential)
+    const float m = value_of(__reduce_max_sync(~0u, chosen >= 0 ? key_of(xe) : 0u));
+    s = a.softmax || m < -40.f ? soft(xe, m) : sigm(xe);
+    if (chosen < 0) s = 0.f;
+    const float sum = warp_sum_of(s);
+    s = sum > 0.f ? s / sum : 0.f;
+  } else if (a.softmax) {
+    if constexpr (!SCORED) top = __shfl_sync(~0u, xe, 0);  // the first choice is the largest logit
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) sum += x[j] > -INFINITY ? soft(x[j], top) : 0.f;
+    sum = warp_sum_of(sum);
+    s = chosen >= 0 ? soft(xe, top) / sum : 0.f;
+  } else {
+    s = chosen >= 0 ? sigm(xe) : 0.f;
   }
   if (lane < a.topk) {
     a.idx[t * a.topk + lane] = chosen;
-    a.p[t * a.topk + lane] = (float)(s * a.factor);
+    a.p[t * a.topk + lane] = s * a.factor;
   }
 }
 
@@ -240,7 +358,7 @@ extern "C" int moe_route_dev(const void* logits, long long ld, int dtype, int ro
   RouteArgs a{};
   a.x = logits; a.bias = bias; a.idx = topk_idx; a.p = topk_p; a.ld = ld; a.rows = rows; a.E = E;
   a.softmax = score == MOE_ROUTE_SOFTMAX; a.groups = keep_group == n_group ? 1 : n_group; a.keep = keep_group;
-  a.group_top = group_top; a.topk = top_k; a.renorm = renorm != 0; a.factor = factor; a.group_size = E / n_group;
+  a.group_top = group_top; a.topk = top_k; a.renorm = renorm != 0; a.factor = (float)factor; a.group_size = E / n_group;
   a.lanes_per_group = 1;
   while (2 * a.lanes_per_group * n_group <= 32) a.lanes_per_group *= 2;
   const bool scored = bias || a.groups > 1;

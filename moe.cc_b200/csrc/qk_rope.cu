@@ -9,12 +9,14 @@
 // with (c, s) = row `position` of the caller's table and R the rotated width;
 // elements from R on pass through. All of it in fp32, each output rounded once.
 //
-// The bound is bytes: every element is read once and written once. A head is
-// held by LPH lanes, each with four elements of the lower half and the four
-// that rotate with them from the upper half, so the rotation needs no
-// exchange between lanes and the mean is a shuffle sum. A block takes one row:
-// its lanes load the weights and the row's table entries once and then walk
-// over the row's heads.
+// The bound is bytes: every element is read once and written once, so the rest
+// has to stay small. A head is held by LPH lanes, each with a run of R elements
+// of the lower half and the R that rotate with them from the upper half: the
+// rotation needs no exchange between lanes and the mean is a shuffle sum. Norm
+// weight and rotation are one pair of factors,
+//   y_lo = inv (x_lo (w_lo c) - x_hi (w_hi s)),  y_hi = inv (x_hi (w_hi c) + x_lo (w_lo s)),
+// which a warp works out once for its row and applies to all the heads that it
+// takes of it: all of them in a long batch, 32 / LPH where rows are few.
 #include "attn.cuh"
 
 namespace moe {
@@ -26,102 +28,179 @@ struct RopeArgs {
   const float *q_norm, *k_norm, *rope;
   const int *row_pos, *row_slot;
   long long ldq, ldk, ldv, ldo, page_stride, token_stride, head_stride;
-  int n_q, n_kv, hd, rot, rope_len, n_slots, page_size;
+  int rows, n_q, n_kv, hd, rot, rope_len, n_slots, page_size;
+  int per_row;            // warps a row
   float eps;
   at::FastDiv page;
 };
 
-constexpr int kThreads = 128;
+constexpr int kWarps = 4;
 
-template <typename TI, typename TO, int LPH>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs a) {
+// R consecutive elements in one or two 16-byte (R = 4 of 16 bits: 8-byte) pieces
+template <typename T, int R> struct Run {
+  typename at::Vec4<T>::raw v[R / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (sizeof(T) == 2 && R == 8) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+    else
+#pragma unroll
+      for (int i = 0; i < R / 4; ++i) v[i] = reinterpret_cast<const typename at::Vec4<T>::raw*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (sizeof(T) == 2 && R == 8) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+    else
+#pragma unroll
+      for (int i = 0; i < R / 4; ++i) reinterpret_cast<typename at::Vec4<T>::raw*>(p)[i] = v[i];
+  }
+  __device__ __forceinline__ void get(float (&f)[R]) const {
+#pragma unroll
+    for (int i = 0; i < R / 4; ++i) at::Vec4<T>::get(v[i], f + 4 * i);
+  }
+  __device__ __forceinline__ void put(const float (&f)[R]) {
+#pragma unroll
+    for (int i = 0; i < R / 4; ++i) v[i] = at::Vec4<T>::put(f + 4 * i);
+  }
+};
+
+// Heads `first`, `first` + step, ... of one row's queries or keys, a warp's
+// 32 / LPH at a time.
+template <typename TI, typename TO, int R, int LPH>
+__device__ __forceinline__ void turn_heads(const RopeArgs& a, const TI* src, TO* dst, long long dst_stride, int heads,
+                                           const float* w, int first, int step, int lo, int hi, bool on, bool turns,
+                                           const float (&c)[R], const float (&s)[R]) {
+  constexpr int kHeads = 32 / LPH;
+  if (first * kHeads >= heads) return;
+  const int g = (threadIdx.x & 31) / LPH;
+  float lc[R], ls[R], hc[R], hs[R];       // w_lo c, w_lo s, w_hi c, w_hi s
+#pragma unroll
+  for (int i = 0; i < R; ++i) { lc[i] = hc[i] = c[i]; ls[i] = hs[i] = s[i]; }
+  if (w && on) {
+    Run<float, R> wl, wh;
+    float l[R], h[R];
+    wl.load(w + lo); wh.load(w + hi);
+    wl.get(l); wh.get(h);
+#pragma unroll
+    for (int i = 0; i < R; ++i) { lc[i] *= l[i]; ls[i] *= l[i]; hc[i] *= h[i]; hs[i] *= h[i]; }
+  }
+  const float inv_hd = 1.0f / (float)a.hd;
+  Run<TI, R> xl, xh;
+  auto fetch = [&](int t) {
+    const int h = t * kHeads + g;
+    if (on && h < heads) { xl.load(src + (long long)h * a.hd + lo); xh.load(src + (long long)h * a.hd + hi); }
+  };
+  fetch(first);
+  for (int t = first; t * kHeads < heads; t += step) {
+    float x[R] = {}, y[R] = {};
+    const int h = t * kHeads + g;
+    const bool live = on && h < heads;
+    if (live) { xl.get(x); xh.get(y); }
+    fetch(t + step);                       // the next heads are on their way meanwhile
+    float inv = 1.0f;
+    if (w) {
+      float sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < R; ++i) sq = fmaf(x[i], x[i], fmaf(y[i], y[i], sq));
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
+      inv = rsqrtf(fmaf(sq, inv_hd, a.eps));
+    }
+    if (!live) continue;
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float e = x[i], o = y[i];
+        x[i] = (e * lc[i] - o * hs[i]) * inv;
+        y[i] = (o * hc[i] + e * ls[i]) * inv;
+      }
+    } else if (w) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) { x[i] *= lc[i] * inv; y[i] *= hc[i] * inv; }
+    }
+    Run<TO, R> out;
+    out.put(x);
+    out.store(dst + h * dst_stride + lo);
+    out.put(y);
+    out.store(dst + h * dst_stride + hi);
+  }
+}
+
+template <typename TI, typename TO, int R, int LPH>
+__global__ void __launch_bounds__(kWarps * 32) qk_norm_rope_kernel(const RopeArgs a) {
   pdl_wait();
   pdl_launch();
-  using VI = at::Vec4<TI>;
-  using VO = at::Vec4<TO>;
-  const int row = blockIdx.x, g = threadIdx.x / LPH, l = threadIdx.x % LPH;
+  constexpr int kHeads = 32 / LPH;
+  // warp `first` of `step` on this row
+  const long long id = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int row = (int)(id / a.per_row), first = (int)(id % a.per_row), step = a.per_row;
+  if (row >= a.rows) return;
+  const int l = threadIdx.x % LPH;
   const int pos = a.row_pos ? a.row_pos[row] : 0;
+  const int slot = a.row_slot ? a.row_slot[row] : -1;
   if (pos < 0 || (a.rot && pos >= a.rope_len)) return;      // a padded row: nothing of it is touched
-  const bool on = 4 * l < a.hd / 2;
-  // this lane's four pairs (lo + t, hi + t)
-  int lo = 4 * l, hi = 4 * l + a.rot / 2;
+  const bool on = R * l < a.hd / 2;
+  // this lane's pairs (lo + i, hi + i)
+  int lo = R * l, hi = R * l + a.rot / 2;
   const bool turns = lo < a.rot / 2;
-  if (!turns) { lo = 4 * l + a.rot / 2; hi = lo + (a.hd - a.rot) / 2; }
-  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (!turns) { lo = R * l + a.rot / 2; hi = lo + (a.hd - a.rot) / 2; }
+  float c[R], s[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) { c[i] = 1.f; s[i] = 0.f; }
   if (on && turns) {
     const float* t = a.rope + (long long)pos * a.rot + lo;
-    at::Vec4<float>::get(*reinterpret_cast<const float4*>(t), c);
-    at::Vec4<float>::get(*reinterpret_cast<const float4*>(t + a.rot / 2), s);
+    Run<float, R> v;
+    v.load(t); v.get(c);
+    v.load(t + a.rot / 2); v.get(s);
   }
-  long long at_slot = -1;
-  if (a.row_slot) {
-    const int slot = a.row_slot[row];
-    if (slot >= 0 && slot < a.n_slots) {
-      const int pg = (int)a.page.div((unsigned)slot);
-      at_slot = pg * a.page_stride + (slot - pg * a.page_size) * a.token_stride;
+  turn_heads<TI, TO, R, LPH>(a, (const TI*)a.q + row * a.ldq, (TO*)a.q_out + row * a.ldo, a.hd, a.n_q, a.q_norm, first, step,
+                             lo, hi, on, turns, c, s);
+  if (slot < 0 || slot >= a.n_slots) return;
+  const int pg = (int)a.page.div((unsigned)slot);
+  const long long to = pg * a.page_stride + (slot - pg * a.page_size) * a.token_stride;
+  // the groups of heads are dealt to the row's warps queries first, then keys, then values
+  const int nq = (a.n_q + kHeads - 1) / kHeads, nk = (a.n_kv + kHeads - 1) / kHeads;
+  const int fk = (first - nq % step + step) % step, fv = (fk - nk % step + step) % step;
+  turn_heads<TI, TO, R, LPH>(a, (const TI*)a.k + row * a.ldk, (TO*)a.kc + to, a.head_stride, a.n_kv, a.k_norm, fk, step,
+                             lo, hi, on, turns, c, s);
+  const int g = (threadIdx.x & 31) / LPH;
+  const TI* v = (const TI*)a.v + row * a.ldv;
+  for (int h = fv * kHeads + g; h < a.n_kv; h += step * kHeads) {
+    if (!on) continue;
+    Run<TI, R> xl, xh;
+    xl.load(v + (long long)h * a.hd + lo);
+    xh.load(v + (long long)h * a.hd + hi);
+    TO* dst = (TO*)a.vc + to + h * a.head_stride;
+    if constexpr (sizeof(TI) == sizeof(TO)) {
+      xl.store((TI*)(dst + lo));
+      xh.store((TI*)(dst + hi));
+    } else {
+      Run<TO, R> out;
+      float x[R];
+      xl.get(x); out.put(x); out.store(dst + lo);
+      xh.get(x); out.put(x); out.store(dst + hi);
     }
-  }
-  const int heads = a.n_q + (at_slot >= 0 ? 2 * a.n_kv : 0);   // without a slot only the queries are worked on
-  const int step = gridDim.y * (kThreads / LPH);
-  int h = blockIdx.y * (kThreads / LPH) + g;
-  // the loop runs alike for all groups of a warp (the sum below shuffles)
-  for (int base = blockIdx.y * (kThreads / LPH); base < heads; base += step, h += step) {
-    const bool live = on && h < heads;
-    const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
-    const int kvh = is_k ? h - a.n_q : h - a.n_q - a.n_kv;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const TI* src = is_q ? (const TI*)a.q + row * a.ldq + (long long)h * a.hd
-                    : is_k ? (const TI*)a.k + row * a.ldk + (long long)kvh * a.hd
-                           : (const TI*)a.v + row * a.ldv + (long long)kvh * a.hd;
-      VI::get(*reinterpret_cast<const typename VI::raw*>(src + lo), x);
-      VI::get(*reinterpret_cast<const typename VI::raw*>(src + hi), x + 4);
-    }
-    float sq = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
-#pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
-    if (!live) continue;
-    const float* w = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-    if (w) {
-      const float inv = 1.0f / sqrtf(sq / (float)a.hd + a.eps);
-      float wl[8];
-      at::Vec4<float>::get(*reinterpret_cast<const float4*>(w + lo), wl);
-      at::Vec4<float>::get(*reinterpret_cast<const float4*>(w + hi), wl + 4);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * wl[i];
-    }
-    if (is_q || is_k) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = x[i], o = x[i + 4];
-        if (turns) {
-          x[i] = e * c[i] - o * s[i];
-          x[i + 4] = o * c[i] + e * s[i];
-        }
-      }
-    }
-    TO* dst = is_q ? (TO*)a.q_out + row * a.ldo + (long long)h * a.hd
-                   : (is_k ? (TO*)a.kc : (TO*)a.vc) + at_slot + kvh * a.head_stride;
-    *reinterpret_cast<typename VO::raw*>(dst + lo) = VO::put(x);
-    *reinterpret_cast<typename VO::raw*>(dst + hi) = VO::put(x + 4);
   }
 }
 
 template <typename TI, typename TO>
-cudaError_t launch_rope(const RopeArgs& a, int rows, cudaStream_t st) {
-  const int heads = a.n_q + 2 * a.n_kv;
+cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
   auto go = [&](auto kernel, int lph) {
-    // few rows: one head per lane group, so that the row spreads over blocks;
-    // many rows: a block keeps its row's table entries for all heads
-    const int per = kThreads / lph, full = (heads + per - 1) / per;
-    const int y = rows >= 1184 ? 1 : full;
-    return launch_pdl(kernel, dim3(rows, y), dim3(kThreads), 0, st, a);
+    // One warp a row where that fills the GPU (16 warps an SM), else as many
+    // as the row has groups of heads
+    const int per = 32 / lph, groups = (a.n_q + per - 1) / per + 2 * ((a.n_kv + per - 1) / per);
+    const long long want = (2368 + a.rows - 1) / a.rows;
+    a.per_row = (int)(want < groups ? want : groups);
+    const long long blocks = ((long long)a.rows * a.per_row + kWarps - 1) / kWarps;
+    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(kWarps * 32), 0, st, a);
   };
-  if (a.hd <= 64) return go(qk_norm_rope_kernel<TI, TO, 8>, 8);
-  if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 16>, 16);
-  return go(qk_norm_rope_kernel<TI, TO, 32>, 32);
+  // runs of 8 where the halves of what rotates and of what does not are whole
+  // numbers of them
+  if (a.rot % 16 == 0 && (a.hd - a.rot) % 16 == 0) {
+    if (a.hd <= 64) return go(qk_norm_rope_kernel<TI, TO, 8, 4>, 4);
+    if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 8, 8>, 8);
+    return go(qk_norm_rope_kernel<TI, TO, 8, 16>, 16);
+  }
+  if (a.hd <= 64) return go(qk_norm_rope_kernel<TI, TO, 4, 8>, 8);
+  if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 4, 16>, 16);
+  return go(qk_norm_rope_kernel<TI, TO, 4, 32>, 32);
 }
 
 // whether the row-strided ranges [p, p + ((rows-1) ld + n) es) of two
@@ -184,15 +263,15 @@ extern "C" int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k,
   a.q_norm = q_norm; a.k_norm = k_norm; a.rope = rope; a.row_pos = row_pos; a.row_slot = row_slot;
   a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
   a.page_stride = cache->page_stride; a.token_stride = cache->token_stride; a.head_stride = cache->head_stride;
-  a.n_q = n_q; a.n_kv = cache->n_kv; a.hd = hd; a.rot = rot_dim; a.rope_len = rope_len;
+  a.rows = rows; a.n_q = n_q; a.n_kv = cache->n_kv; a.hd = hd; a.rot = rot_dim; a.rope_len = rope_len;
   a.n_slots = cache->n_pages * cache->page_size; a.page_size = cache->page_size; a.eps = eps;
   a.page = at::FastDiv((unsigned)cache->page_size);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
-  if (dtype == MOE_DTYPE_BF16) e = launch_rope<__nv_bfloat16, __nv_bfloat16>(a, rows, st);
-  else if (dtype == MOE_DTYPE_F16) e = launch_rope<__half, __half>(a, rows, st);
-  else if (cache->dtype == MOE_DTYPE_F32) e = launch_rope<float, float>(a, rows, st);
-  else if (cache->dtype == MOE_DTYPE_BF16) e = launch_rope<float, __nv_bfloat16>(a, rows, st);
-  else e = launch_rope<float, __half>(a, rows, st);
+  if (dtype == MOE_DTYPE_BF16) e = launch_rope<__nv_bfloat16, __nv_bfloat16>(a, st);
+  else if (dtype == MOE_DTYPE_F16) e = launch_rope<__half, __half>(a, st);
+  else if (cache->dtype == MOE_DTYPE_F32) e = launch_rope<float, float>(a, st);
+  else if (cache->dtype == MOE_DTYPE_BF16) e = launch_rope<float, __nv_bfloat16>(a, st);
+  else e = launch_rope<float, __half>(a, st);
   return at::launched(e, who);
 }

@@ -1,6 +1,9 @@
 """GPU: expert routing from given logits against a plain 64-bit form. The
-chosen experts have to be equal; a weight is one fp32 rounding (2^-24) of a
-64-bit value."""
+chosen experts have to be equal. A weight is computed in fp32, in units of
+2^-24: exp errs by 4 (2 ulp) and by z, its rounded argument (x minus the
+largest chosen, or of all, logit), a sigmoid by 5; the sum it is divided by by
+as much, and by its additions (5 over the warp, 32 more and the mean of z, below
+8, where it runs over all experts); the quotient and the factor by 2."""
 import math
 
 import numpy as np
@@ -58,7 +61,14 @@ def check(x, k, bias=None, score="softmax", groups=1, keep=1, group_top=1, renor
     want_i, want_p = route_reference(x.float().cpu().numpy(), None if bias is None else bias.cpu().numpy(), score, groups, keep,
                                      group_top, k, renorm, factor)
     assert np.array_equal(idx.cpu().numpy(), want_i)
-    err = np.abs(p.cpu().numpy() - want_p) - (2.0**-24 + 1e-13) * np.abs(want_p) - 1e-45
+    xs = np.take_along_axis(x.double().cpu().numpy(), np.maximum(want_i, 0).astype(np.int64), 1)
+    seen = np.where((want_i >= 0) & np.isfinite(xs), xs, -np.inf)
+    high = np.where(np.isnan(x.double().cpu().numpy()), -np.inf, x.double().cpu().numpy()).max(1, keepdims=True) \
+        if score == "softmax" and not renorm else seen.max(1, keepdims=True)
+    with np.errstate(invalid="ignore"):
+        z = np.nan_to_num(np.clip(high - seen, 0, 1e4), nan=0.0, posinf=1e4).max(1, keepdims=True)
+    units = 2 * (z + 5) + (45 if not renorm else 5) + 2
+    err = np.abs(p.cpu().numpy() - want_p) - units * 2.0**-24 * np.abs(want_p) - factor * 2.0**-126
     assert (err <= 0).all(), float(err.max())
     return idx, p
 
@@ -119,6 +129,28 @@ def test_near_ties_are_ordered_in_64_bits(gpu):
     for bias in (None, torch.full((64,), 3.0).cuda()):
         idx, _ = check(x.cuda(), 3, bias, "sigmoid")
         assert idx[0].tolist() == [20, 50, 0]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_many_tokens_choose_as_64_bits_do(gpu, score):
+    """A balance bias over scores that lie close: thousands of tokens, some of
+    which fp32 cannot rank."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    x = 0.02 * torch.randn(3000, 256, generator=g, device="cuda")
+    check(x, 8, 0.001 * torch.randn(256, generator=g, device="cuda"), score, 8, 4, 2)
+    check(x[:500], 8, None, score, 8, 4, 2)
+    check(x[:500] + 12, 8, torch.zeros(256, device="cuda"), score, 1, 1, 1)
+
+
+def test_ratios_survive_where_scores_underflow(gpu):
+    x = torch.full((2, 32), -300.0)
+    x[0, 3], x[0, 4], x[1, 5] = -299.0, -299.5, 200.0
+    for score in ("sigmoid", "softmax"):
+        check(x.cuda(), 4, None, score)
+    bias = torch.zeros(32)
+    bias[8:12] = 5.0                                # the chosen are not the likely ones
+    check(x.cuda(), 4, bias.cuda(), "softmax")
 
 
 def test_strided_rows_another_stream_and_repeat(gpu):

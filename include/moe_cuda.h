@@ -392,7 +392,7 @@ int moe_kv_plan_dev(const int* past_len, const int* new_len, int n_seq,
  * be any. q_out may be q, with the same type and stride; it must not overlap
  * q, k or v otherwise. n_q may be 0 (keys and values only), row_slot NULL
  * (queries only). A row whose position is negative or not below rope_len is
- * padding: nothing of it is read or written. A slot outside the cache appends
+ * padding: nothing of it is written. A slot outside the cache appends
  * nothing. Rows must have different slots. */
 int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k, long long ldk,
                          const void* v, long long ldv, int dtype, int rows, int n_q,

@@ -14,11 +14,11 @@
 // round to the same number often enough to change which expert is chosen.
 // Without a bias or groups the order of the scores is the order of the logits,
 // exactly, and no score is needed for it. Otherwise a token is first ranked by
-// fp32 scores, whose error is bounded (`margin`); where two neighbours of the
-// ranking, the last chosen and the first left out included, or the groups on
-// either side of the cut, are closer than that, the token is ranked again by
-// scores in 64 bits. About 1 token in 100 is. The weights are fp32 softmax or
-// sigmoid values of the chosen.
+// fp32 scores, whose error is bounded (`margin`): the list of the best goes on
+// past top_k until the next is clearly behind, and if two neighbours in it are
+// closer than the bound, its few experts are ordered again by scores in 64 bits.
+// Where the groups on either side of the cut are that close, the whole token is
+// ranked again in 64 bits. The weights are fp32 softmax or sigmoid values.
 //
 // One warp routes one token: expert j * 32 + lane in lane `lane`. A round of
 // the selection takes the largest key by a warp reduction, then the lowest
@@ -41,6 +41,7 @@ struct RouteArgs {
   float* p;
   long long ld;
   int rows, E, softmax, groups, keep, group_top, topk, renorm, lanes_per_group, group_size;
+  at::FastDiv group;
   float factor;
 };
 
@@ -106,11 +107,16 @@ __device__ __forceinline__ void choices(const RouteArgs& a, const float (&x)[EPL
 
 // How far apart two fp32 choices must be for the exact ones to be ordered
 // alike. In units of 2^-24: a sigmoid errs by 4 (expf by 2 ulp, damped by
-// e^-x s < 1, sum and quotient); a softmax score relatively by |z| (its rounded
+// e^-x s < 1, sum and quotient), with the bias by |c| more, two of them by less
+// than 2^4 (1 + |u| + |v|); a softmax score relatively by |z| (its rounded
 // argument z = x - max; |z| s < 0.4), 4 (expf), 2 (quotient and product) and by
-// its sum: up to 37 roundings and the mean of |z|, below ln 1024 + 1; together
-// less than 2^6. A sum with the bias adds its own rounding. Two of them: 2^-17.
-__device__ __forceinline__ float margin(float u, float v) { return 0x1p-17f * (1.0f + fabsf(u) + fabsf(v)); }
+// its sum, up to 37 roundings and the mean of |z|, below ln 1024 + 1: less than
+// 2^6, two of them and the bias 2^7 (1 + |u| + |v|). `drop`: the low bits of
+// either that were taken out, relatively 2^(drop - 23).
+__device__ __forceinline__ float margin(const RouteArgs& a, float u, float v, float drop) {
+  const float m = fabsf(u) + fabsf(v);
+  return fmaf(m, drop, (a.softmax ? 0x1p-17f : 0x1p-20f) * (1.0f + m));
+}
 
 // Takes the experts outside the `keep` best groups out of c. cut[0], cut[1]:
 // the least sum that stays and the largest that does not.
@@ -148,7 +154,7 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, F* mine, F (&c)[
   cut[1] = __shfl_sync(~0u, gs, __ffs(__ballot_sync(~0u, head && before == a.keep)) - 1);
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
-    const int e = j * 32 + lane, ge = e / a.group_size;
+    const int e = j * 32 + lane, ge = (int)a.group.div((unsigned)e);
     if (e < a.E && !((stays >> (ge * lpg)) & 1)) c[j] = -INFINITY;
   }
 }
@@ -211,6 +217,38 @@ __device__ __noinline__ int choose64(const RouteArgs& a, const float (&x)[EPL], 
   return chosen;
 }
 
+// The n experts that lanes 0 .. n - 1 list, in the order of their choices in
+// 64 bits; lane r returns the r-th.
+template <typename T, int EPL>
+__device__ __noinline__ int order64(const RouteArgs& a, const float (&x)[EPL], float top, long long t, int listed, int n) {
+  const int lane = threadIdx.x & 31;
+  double total = 1.0;
+  if (a.softmax && a.bias) {                    // without a bias the sum orders nothing
+    total = 0.0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) total += x[j] > -INFINITY ? soft64(x[j], top) : 0.0;
+    total = warp_sum_of(total);
+  }
+  double c = 0.0;
+  if (lane < n) {
+    const float xe = logit<T>(a.x, t * a.ld + listed);
+    c = a.softmax ? soft64(xe, top) / total : sigm64(xe);
+    if (a.bias) c += (double)a.bias[listed];
+  }
+  int rank = 0;
+  for (int m = 0; m < n; ++m) {
+    const double v = __shfl_sync(~0u, c, m);
+    const int e = __shfl_sync(~0u, listed, m);
+    rank += v > c || (v == c && e < listed);
+  }
+  int chosen = -1;
+  for (int m = 0; m < n; ++m) {
+    const int r = __shfl_sync(~0u, rank, m), e = __shfl_sync(~0u, listed, m);
+    if (r == lane) chosen = e;
+  }
+  return chosen;
+}
+
 // EPL experts a lane; SCORED: the choice needs every score (bias or groups)
 template <typename T, int EPL, bool SCORED>
 __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteArgs a) {
@@ -238,20 +276,37 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
     float c[EPL], cut[2] = {INFINITY, -INFINITY};
     choices<float, EPL>(a, x, top, c);
     if (a.groups > 1) keep_groups<float, EPL>(a, (float*)(choice_sm + warp * (EPL * 32)), c, cut);
+    // Keys: the fp32 choice without its lowest bits, which hold the index from
+    // the top down. The list runs on past top_k until the next one is clearly
+    // behind; then nothing outside it can belong in it.
+    constexpr unsigned kLow = EPL * 32 - 1;
+    constexpr float kDrop = (float)(EPL * 32) * 0x1p-23f;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) key[j] = c[j] > -INFINITY ? key_of(c[j]) : 0u;
+    for (int j = 0; j < EPL; ++j)
+      key[j] = c[j] > -INFINITY ? (key_of(c[j]) & ~kLow) | (kLow - (j * 32 + lane)) : 0u;
     float last = INFINITY;
-    bool close = cut[0] - cut[1] < 2 * margin(cut[0], cut[1]);
-    for (int r = 0; r <= a.topk; ++r) {                    // one more than is taken: the first left out
-      unsigned k;
-      const int e = take<EPL>(key, k);
-      if (e < 0) break;
-      const float v = value_of(k);
-      close |= !(last - v >= margin(last, v));
+    int n = 0;
+    bool unsure = false, anew = a.groups > 1 && cut[0] - cut[1] < 2 * margin(a, cut[0], cut[1], 0.f);
+    for (;;) {
+      unsigned best = key[0];
+#pragma unroll
+      for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
+      best = __reduce_max_sync(~0u, best);
+      if (best == 0u) break;
+      const float v = value_of(best & ~kLow);
+      const bool near = !(last - v >= margin(a, last, v, kDrop));
+      if (n >= a.topk && !near) break;
+      unsure |= near;
+      if (n == 32) { anew = true; break; }
+      if (lane == n) chosen = (int)(kLow - (best & kLow));
+      ++n;
       last = v;
-      if (lane == r && r < a.topk) chosen = e;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) key[j] = key[j] == best ? 0u : key[j];
     }
-    if (close) chosen = choose64<EPL>(a, x, top, choice_sm + warp * (EPL * 32));
+    if (anew) chosen = choose64<EPL>(a, x, top, choice_sm + warp * (EPL * 32));
+    else if (unsure) chosen = order64<T, EPL>(a, x, top, t, chosen, n);
+    if (lane >= a.topk) chosen = -1;
   } else if constexpr (sizeof(T) == 2) {
     // the logit's 16 bits above, the index from the top down below them
 #pragma unroll
@@ -359,6 +414,7 @@ extern "C" int moe_route_dev(const void* logits, long long ld, int dtype, int ro
   a.x = logits; a.bias = bias; a.idx = topk_idx; a.p = topk_p; a.ld = ld; a.rows = rows; a.E = E;
   a.softmax = score == MOE_ROUTE_SOFTMAX; a.groups = keep_group == n_group ? 1 : n_group; a.keep = keep_group;
   a.group_top = group_top; a.topk = top_k; a.renorm = renorm != 0; a.factor = (float)factor; a.group_size = E / n_group;
+  a.group = at::FastDiv((unsigned)(E / n_group));
   a.lanes_per_group = 1;
   while (2 * a.lanes_per_group * n_group <= 32) a.lanes_per_group *= 2;
   const bool scored = bias || a.groups > 1;

@@ -10,27 +10,30 @@
 // belongs to the sequence whose inclusive sum of new lengths first exceeds i.
 //
 // Nothing here is bound by bytes (a 32-sequence decode step reads and writes
-// about a kilobyte): the time is one launch and a chain of dependent loads.
-// So every CTA scans all lengths for itself in shared memory rather than
-// waiting for another CTA's scan, and rows and pages are then spread evenly
-// over the threads, each finding its sequence by bisection: a long prompt
-// costs no single warp more than the others. Large plans run as one cluster
-// of 8 CTAs, whose barrier (after every CTA has read its inputs) is what lets
-// kv_len and free_head be updated in place.
+// about a kilobyte): the time is a launch and a chain of dependent loads. So
+// every CTA scans all lengths for itself in shared memory rather than waiting
+// for another CTA's scan, and rows and pages are then spread evenly over all
+// threads, which find their sequences by bisection: a long prompt costs no
+// single warp more than the others.
+//
+// kv_len may be past_len and free_head_out free_head. With one CTA a barrier
+// between reading and writing does for that; with several, another launch of
+// one CTA writes them when all have read.
 #include "attn.cuh"
 
 namespace moe {
 namespace {
 
 constexpr int kMaxSeqs = 16384;      // 12 bytes of shared memory each
-constexpr int kMaxThreads = 1024;
-constexpr int kCluster = 8;
+constexpr int kMaxThreads = 512;
 
 struct PlanArgs {
   const int *past_len, *new_len, *free_pages, *free_head;
   int *table, *kv_len, *row_seq, *row_pos, *row_slot, *head_out, *status;
   long long table_stride;
   int n_seq, page_size, n_pages, n_free, max_pages, row_cap;
+  int quads;              // rows are taken four at a time
+  int plan, sums;         // whether this launch writes pages and rows; kv_len, free_head_out and status
   at::FastDiv page;
 };
 
@@ -95,46 +98,74 @@ __global__ void __launch_bounds__(kMaxThreads) kv_plan_kernel(const PlanArgs a) 
   const int r1 = __shfl_up_sync(~0u, r, 1), g1 = __shfl_up_sync(~0u, g, 1);
   if (lane) { r0 = sat_add(r0, r1); g0 += g1; }
   for (int s = s0; s < s1; ++s) { row_end[s] = sat_add(row_end[s], r0); page_end[s] += g0; }
-  // all CTAs have read past_len, new_len and free_head before any of their
-  // in-place successors is written
-  if (ctas > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
   __syncthreads();
 
   const unsigned first = cta * nt + tid, step = ctas * nt;
   const int taken = min(all_pages, a.n_free - head);
+  if (a.sums && cta == 0) {
+    if (a.kv_len)
+      for (int s = tid; s < a.n_seq; s += nt) a.kv_len[s] = past[s] + (row_end[s] - (s ? row_end[s - 1] : 0));
+    if (tid == 0) {
+      if (a.head_out) *a.head_out = head + taken;
+      if (a.status) { a.status[0] = all_rows; a.status[1] = all_pages; a.status[2] = taken; }
+    }
+  }
+  if (!a.plan) return;
   for (unsigned j = first; j < (unsigned)all_pages; j += step) {
     const int s = owner_of(page_end, a.n_seq, (int)j), start = s ? page_end[s - 1] : 0;
     a.table[s * a.table_stride + pages_of(a, past[s]) + ((int)j - start)] = (int)j < taken ? a.free_pages[head + j] : -1;
   }
-  for (unsigned i = first; i < (unsigned)a.row_cap; i += step) {
-    int seq = -1, pos = -1, slot = -1;
-    if (i < (unsigned)all_rows) {
-      seq = owner_of(row_end, a.n_seq, (int)i);
-      pos = past[seq] + ((int)i - (seq ? row_end[seq - 1] : 0));
-      const int pi = (int)a.page.div((unsigned)pos), held = pages_of(a, past[seq]);
-      if (pi < a.max_pages) {
-        int pg = -1;
-        if (pi < held) pg = a.table[seq * a.table_stride + pi];
-        else {
-          const int j = (seq ? page_end[seq - 1] : 0) + (pi - held);
-          if (j < taken) pg = a.free_pages[head + j];
-        }
-        if (pg >= 0 && pg < a.n_pages) slot = pg * a.page_size + (pos - pi * a.page_size);
+  // row i of sequence s
+  auto row_of = [&](int i, int s, int& pos, int& slot) {
+    pos = past[s] + (i - (s ? row_end[s - 1] : 0));
+    const int pi = (int)a.page.div((unsigned)pos), held = pages_of(a, past[s]);
+    int pg = -1;
+    if (pi < a.max_pages) {
+      if (pi < held) pg = a.table[s * a.table_stride + pi];
+      else {
+        const int j = (s ? page_end[s - 1] : 0) + (pi - held);
+        if (j < taken) pg = a.free_pages[head + j];
       }
     }
-    a.row_seq[i] = seq;
-    a.row_pos[i] = pos;
-    a.row_slot[i] = slot;
+    slot = pg >= 0 && pg < a.n_pages ? pg * a.page_size + (pos - pi * a.page_size) : -1;
+  };
+  if (!a.quads) {
+    for (unsigned i = first; i < (unsigned)a.row_cap; i += step) {
+      int s = -1, pos = -1, slot = -1;
+      if (i < (unsigned)all_rows) {
+        s = owner_of(row_end, a.n_seq, (int)i);
+        row_of((int)i, s, pos, slot);
+      }
+      a.row_seq[i] = s;
+      a.row_pos[i] = pos;
+      a.row_slot[i] = slot;
+    }
+    return;
   }
-  if (a.kv_len)
-    for (unsigned s = first; s < (unsigned)a.n_seq; s += step)
-      a.kv_len[s] = past[s] + (row_end[s] - (s ? row_end[s - 1] : 0));
-  if (first == 0) {
-    if (a.head_out) *a.head_out = head + taken;
-    if (a.status) { a.status[0] = all_rows; a.status[1] = all_pages; a.status[2] = taken; }
+  // Four consecutive rows a thread: one search for the first of them, then on
+  // from sequence to sequence.
+  for (unsigned i0 = 4 * first; i0 < (unsigned)a.row_cap; i0 += 4 * step) {
+    int seq[4] = {-1, -1, -1, -1}, pos[4] = {-1, -1, -1, -1}, slot[4] = {-1, -1, -1, -1};
+    if (i0 < (unsigned)all_rows) {
+      int s = owner_of(row_end, a.n_seq, (int)i0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = (int)(i0 + k);
+        if (i0 + k >= (unsigned)all_rows) break;
+        while (row_end[s] <= i) ++s;
+        seq[k] = s;
+        row_of(i, s, pos[k], slot[k]);
+      }
+    }
+    if (i0 + 4 <= (unsigned)a.row_cap) {
+      *reinterpret_cast<int4*>(a.row_seq + i0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+      *reinterpret_cast<int4*>(a.row_pos + i0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<int4*>(a.row_slot + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i0 + k < (unsigned)a.row_cap) { a.row_seq[i0 + k] = seq[k]; a.row_pos[i0 + k] = pos[k]; a.row_slot[i0 + k] = slot[k]; }
+    }
   }
 }
 
@@ -172,30 +203,25 @@ extern "C" int moe_kv_plan_dev(const int* past_len, const int* new_len, int n_se
   a.head_out = free_head_out; a.status = status; a.table_stride = max_pages;
   a.n_seq = n_seq; a.page_size = page_size; a.n_pages = n_pages; a.n_free = n_free; a.max_pages = max_pages;
   a.row_cap = row_cap; a.page = at::FastDiv((unsigned)page_size);
-  const int work = n_seq > row_cap ? n_seq : row_cap;
-  const int threads = work <= 256 ? 256 : kMaxThreads, ctas = work <= 2 * kMaxThreads ? 1 : kCluster;
+  // one row a thread up to 2048 (latency), four in large plans
+  a.quads = row_cap > 2048 && ((uintptr_t)row_seq | (uintptr_t)row_pos | (uintptr_t)row_slot) % 16 == 0;
+  const int work = n_seq > row_cap ? n_seq : row_cap, each = kMaxThreads * (a.quads ? 4 : 1);
+  const int threads = work <= 256 ? 256 : kMaxThreads;
+  const int ctas = work <= 2 * kMaxThreads ? 1 : work / each < 148 ? (work + each - 1) / each : 148;
+  const bool in_place = ctas > 1 && ((kv_len && kv_len == past_len) || (free_head_out && free_head_out == free_head));
   const size_t smem = sizeof(int) * 3 * (size_t)n_seq;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)(sizeof(int) * 3 * kMaxSeqs));
     if (e != cudaSuccess) return at::fail(MOE_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attrs[2];
-  int n = 0;
-  if (pdl_enabled()) {
-    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[n++].val.programmaticStreamSerializationAllowed = 1;
+  a.plan = 1;
+  a.sums = !in_place;
+  cudaError_t e = launch_pdl(kv_plan_kernel, dim3(ctas), dim3(threads), smem, (cudaStream_t)stream, a);
+  if (e == cudaSuccess && in_place) {
+    a.plan = 0;
+    a.sums = 1;
+    e = launch_pdl(kv_plan_kernel, dim3(1), dim3(threads), smem, (cudaStream_t)stream, a);
   }
-  if (ctas > 1) {
-    attrs[n].id = cudaLaunchAttributeClusterDimension;
-    attrs[n].val.clusterDim.x = ctas; attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  cfg.attrs = attrs;
-  cfg.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_plan_kernel, a);
   return at::launched(e, who);
 }

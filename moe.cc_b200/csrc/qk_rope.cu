@@ -61,132 +61,170 @@ template <typename T, int R> struct Run {
   }
 };
 
-// Heads `first`, `first` + step, ... of one row's queries or keys, a warp's
-// 32 / LPH at a time.
-template <typename TI, typename TO, int R, int LPH>
-__device__ __forceinline__ void turn_heads(const RopeArgs& a, const TI* src, TO* dst, long long dst_stride, int heads,
-                                           const float* w, int first, int step, int lo, int hi, bool on, bool turns,
-                                           const float (&c)[R], const float (&s)[R]) {
+// Two fp32 operations an instruction.
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 pack(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack(F2 p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v)); }
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// FULL: the lanes of a head hold it exactly, all of it rotated.
+template <typename TI, typename TO, int R, int LPH, bool FULL>
+__global__ void __launch_bounds__(kWarps * 32, sizeof(TI) == 2 ? 5 : 4) qk_norm_rope_kernel(const RopeArgs a) {
+  pdl_wait();
+  pdl_launch();
   constexpr int kHeads = 32 / LPH;
-  if (first * kHeads >= heads) return;
-  const int g = (threadIdx.x & 31) / LPH;
-  float lc[R], ls[R], hc[R], hs[R];       // w_lo c, w_lo s, w_hi c, w_hi s
-#pragma unroll
-  for (int i = 0; i < R; ++i) { lc[i] = hc[i] = c[i]; ls[i] = hs[i] = s[i]; }
-  if (w && on) {
-    Run<float, R> wl, wh;
-    float l[R], h[R];
-    wl.load(w + lo); wh.load(w + hi);
-    wl.get(l); wh.get(h);
-#pragma unroll
-    for (int i = 0; i < R; ++i) { lc[i] *= l[i]; ls[i] *= l[i]; hc[i] *= h[i]; hs[i] *= h[i]; }
-  }
-  const float inv_hd = 1.0f / (float)a.hd;
-  Run<TI, R> xl, xh;
-  auto fetch = [&](int t) {
-    const int h = t * kHeads + g;
-    if (on && h < heads) { xl.load(src + (long long)h * a.hd + lo); xh.load(src + (long long)h * a.hd + hi); }
+  const long long id = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int row = (int)(id / a.per_row), step = a.per_row, me = (int)(id - (long long)row * step);
+  if (row >= a.rows) return;
+  const int hd = FULL ? 2 * R * LPH : a.hd, rot = FULL ? hd : a.rot;
+  const int l = threadIdx.x % LPH, g = (threadIdx.x & 31) / LPH;
+  const bool on = FULL || R * l < hd / 2, turns = FULL || R * l < rot / 2;
+  // this lane's pairs (lo + i, hi + i)
+  int lo = R * l, hi = R * l + rot / 2;
+  if (!turns) { lo = R * l + rot / 2; hi = lo + (hd - rot) / 2; }
+  if (!on) lo = hi = 0;
+
+  // The row's groups of kHeads heads, values, keys and queries, are dealt to
+  // its warps. The first of each are on their way before anything is known of
+  // the row. A lane past the last head repeats the last one and stores nothing.
+  const int nk = a.row_slot ? (a.n_kv + kHeads - 1) / kHeads : 0, nq = (a.n_q + kHeads - 1) / kHeads;
+  const int fk = (me - nk % step + step) % step, fq = (me - 2 * nk % step + step) % step;
+  struct Pair { Run<TI, R> lo, hi; };
+  auto fetch = [&](const TI* base, int t, int heads) {
+    Pair r;
+    const TI* p = base + min(t * kHeads + g, heads - 1) * hd;
+    r.lo.load(p + lo);
+    r.hi.load(p + hi);
+    return r;
   };
-  fetch(first);
-  for (int t = first; t * kHeads < heads; t += step) {
-    float x[R] = {}, y[R] = {};
-    const int h = t * kHeads + g;
-    const bool live = on && h < heads;
-    if (live) { xl.get(x); xh.get(y); }
-    fetch(t + step);                       // the next heads are on their way meanwhile
+  const TI *qrow = (const TI*)a.q + row * a.ldq, *krow = (const TI*)a.k + row * a.ldk, *vrow = (const TI*)a.v + row * a.ldv;
+  Pair pv, pk, p0, p1;
+  if (me < nk) pv = fetch(vrow, me, a.n_kv);
+  if (fk < nk) pk = fetch(krow, fk, a.n_kv);
+  if (fq < nq) p0 = fetch(qrow, fq, a.n_q);
+  if (fq + step < nq) p1 = fetch(qrow, fq + step, a.n_q);
+  const int pos = a.row_pos ? a.row_pos[row] : 0;
+  const int slot = a.row_slot ? a.row_slot[row] : -1;
+  if (pos < 0 || (rot && pos >= a.rope_len)) return;        // a padded row: nothing of it is written
+  const float* cs = a.rope + (turns ? (long long)pos * rot + lo : 0);
+
+  F2 lc[R / 2], ls[R / 2], hc[R / 2], hs[R / 2];       // w_lo c, w_lo s, w_hi c, -w_hi s
+  auto factors = [&](const float* w) {
+    float c[R], s[R], u[R], v[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) { c[i] = u[i] = v[i] = 1.f; s[i] = 0.f; }
+    Run<float, R> f;
+    if (turns) { f.load(cs); f.get(c); f.load(cs + rot / 2); f.get(s); }
+    if (w) { f.load(w + lo); f.get(u); f.load(w + hi); f.get(v); }
+#pragma unroll
+    for (int i = 0; i < R; i += 2) {
+      lc[i / 2] = pack(c[i] * u[i], c[i + 1] * u[i + 1]);
+      ls[i / 2] = pack(s[i] * u[i], s[i + 1] * u[i + 1]);
+      hc[i / 2] = pack(c[i] * v[i], c[i + 1] * v[i + 1]);
+      hs[i / 2] = pack(-s[i] * v[i], -s[i + 1] * v[i + 1]);
+    }
+  };
+  const float inv_hd = 1.0f / (float)hd;
+  auto turn = [&](const Pair& r, const float* w, TO* dst, bool store) {
+    float x[R], y[R];
+    r.lo.get(x);
+    r.hi.get(y);
+    F2 X[R / 2], Y[R / 2];
+#pragma unroll
+    for (int i = 0; i < R; i += 2) { X[i / 2] = pack(x[i], x[i + 1]); Y[i / 2] = pack(y[i], y[i + 1]); }
     float inv = 1.0f;
     if (w) {
-      float sq = 0.f;
+      F2 s = mul(X[0], X[0]);
 #pragma unroll
-      for (int i = 0; i < R; ++i) sq = fmaf(x[i], x[i], fmaf(y[i], y[i], sq));
+      for (int i = 1; i < R / 2; ++i) s = fma(X[i], X[i], s);
+#pragma unroll
+      for (int i = 0; i < R / 2; ++i) s = fma(Y[i], Y[i], s);
+      float s0, s1;
+      unpack(s, s0, s1);
+      float sq = on ? s0 + s1 : 0.f;
 #pragma unroll
       for (int o = LPH / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
       inv = rsqrtf(fmaf(sq, inv_hd, a.eps));
     }
-    if (!live) continue;
-    if (turns) {
+    if (!on || !store) return;
+    if (turns || w) {
+      const F2 n = pack(inv, inv);
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const float e = x[i], o = y[i];
-        x[i] = (e * lc[i] - o * hs[i]) * inv;
-        y[i] = (o * hc[i] + e * ls[i]) * inv;
+      for (int i = 0; i < R / 2; ++i) {
+        F2 u = mul(X[i], lc[i]), v = mul(Y[i], hc[i]);
+        if (turns) { u = fma(Y[i], hs[i], u); v = fma(X[i], ls[i], v); }
+        unpack(mul(u, n), x[2 * i], x[2 * i + 1]);
+        unpack(mul(v, n), y[2 * i], y[2 * i + 1]);
       }
-    } else if (w) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) { x[i] *= lc[i] * inv; y[i] *= hc[i] * inv; }
     }
     Run<TO, R> out;
     out.put(x);
-    out.store(dst + h * dst_stride + lo);
+    out.store(dst + lo);
     out.put(y);
-    out.store(dst + h * dst_stride + hi);
-  }
-}
+    out.store(dst + hi);
+  };
 
-template <typename TI, typename TO, int R, int LPH>
-__global__ void __launch_bounds__(kWarps * 32) qk_norm_rope_kernel(const RopeArgs a) {
-  pdl_wait();
-  pdl_launch();
-  constexpr int kHeads = 32 / LPH;
-  // warp `first` of `step` on this row
-  const long long id = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int row = (int)(id / a.per_row), first = (int)(id % a.per_row), step = a.per_row;
-  if (row >= a.rows) return;
-  const int l = threadIdx.x % LPH;
-  const int pos = a.row_pos ? a.row_pos[row] : 0;
-  const int slot = a.row_slot ? a.row_slot[row] : -1;
-  if (pos < 0 || (a.rot && pos >= a.rope_len)) return;      // a padded row: nothing of it is touched
-  const bool on = R * l < a.hd / 2;
-  // this lane's pairs (lo + i, hi + i)
-  int lo = R * l, hi = R * l + a.rot / 2;
-  const bool turns = lo < a.rot / 2;
-  if (!turns) { lo = R * l + a.rot / 2; hi = lo + (a.hd - a.rot) / 2; }
-  float c[R], s[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) { c[i] = 1.f; s[i] = 0.f; }
-  if (on && turns) {
-    const float* t = a.rope + (long long)pos * a.rot + lo;
-    Run<float, R> v;
-    v.load(t); v.get(c);
-    v.load(t + a.rot / 2); v.get(s);
-  }
-  turn_heads<TI, TO, R, LPH>(a, (const TI*)a.q + row * a.ldq, (TO*)a.q_out + row * a.ldo, a.hd, a.n_q, a.q_norm, first, step,
-                             lo, hi, on, turns, c, s);
-  if (slot < 0 || slot >= a.n_slots) return;
-  const int pg = (int)a.page.div((unsigned)slot);
-  const long long to = pg * a.page_stride + (slot - pg * a.page_size) * a.token_stride;
-  // the groups of heads are dealt to the row's warps queries first, then keys, then values
-  const int nq = (a.n_q + kHeads - 1) / kHeads, nk = (a.n_kv + kHeads - 1) / kHeads;
-  const int fk = (first - nq % step + step) % step, fv = (fk - nk % step + step) % step;
-  turn_heads<TI, TO, R, LPH>(a, (const TI*)a.k + row * a.ldk, (TO*)a.kc + to, a.head_stride, a.n_kv, a.k_norm, fk, step,
-                             lo, hi, on, turns, c, s);
-  const int g = (threadIdx.x & 31) / LPH;
-  const TI* v = (const TI*)a.v + row * a.ldv;
-  for (int h = fv * kHeads + g; h < a.n_kv; h += step * kHeads) {
-    if (!on) continue;
-    Run<TI, R> xl, xh;
-    xl.load(v + (long long)h * a.hd + lo);
-    xh.load(v + (long long)h * a.hd + hi);
-    TO* dst = (TO*)a.vc + to + h * a.head_stride;
-    if constexpr (sizeof(TI) == sizeof(TO)) {
-      xl.store((TI*)(dst + lo));
-      xh.store((TI*)(dst + hi));
-    } else {
-      Run<TO, R> out;
-      float x[R];
-      xl.get(x); out.put(x); out.store(dst + lo);
-      xh.get(x); out.put(x); out.store(dst + hi);
+  if (slot >= 0 && slot < a.n_slots) {
+    const int pg = (int)a.page.div((unsigned)slot);
+    const long long to = pg * a.page_stride + (slot - pg * a.page_size) * a.token_stride;
+    for (int t = me; t < nk; t += step) {                   // values: as they are, in the cache's type
+      if (t != me) pv = fetch(vrow, t, a.n_kv);
+      const int h = t * kHeads + g;
+      if (!on || h >= a.n_kv) continue;
+      TO* dst = (TO*)a.vc + to + h * a.head_stride;
+      if constexpr (sizeof(TI) == sizeof(TO)) {
+        pv.lo.store((TI*)(dst + lo));
+        pv.hi.store((TI*)(dst + hi));
+      } else {
+        Run<TO, R> out;
+        float x[R];
+        pv.lo.get(x); out.put(x); out.store(dst + lo);
+        pv.hi.get(x); out.put(x); out.store(dst + hi);
+      }
     }
+    if (fk < nk) factors(a.k_norm);
+    for (int t = fk; t < nk; t += step) {
+      if (t != fk) pk = fetch(krow, t, a.n_kv);
+      const int h = t * kHeads + g;
+      turn(pk, a.k_norm, (TO*)a.kc + to + h * a.head_stride, h < a.n_kv);
+    }
+  }
+  if (fq >= nq) return;
+  factors(a.q_norm);
+  TO* dst = (TO*)a.q_out + row * a.ldo + (fq * kHeads + g) * hd;
+  for (int t = fq; t < nq; t += 2 * step) {                 // two groups on their way while two are worked on
+    turn(p0, a.q_norm, dst, t * kHeads + g < a.n_q);
+    dst += step * kHeads * hd;
+    if (t + 2 * step < nq) p0 = fetch(qrow, t + 2 * step, a.n_q);
+    if (t + step >= nq) break;
+    turn(p1, a.q_norm, dst, (t + step) * kHeads + g < a.n_q);
+    dst += step * kHeads * hd;
+    if (t + 3 * step < nq) p1 = fetch(qrow, t + 3 * step, a.n_q);
   }
 }
 
 template <typename TI, typename TO>
 cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
   auto go = [&](auto kernel, int lph) {
-    // One warp a row where that fills the GPU (16 warps an SM), else as many
-    // as the row has groups of heads
-    const int per = 32 / lph, groups = (a.n_q + per - 1) / per + 2 * ((a.n_kv + per - 1) / per);
-    const long long want = (2368 + a.rows - 1) / a.rows;
+    // One warp a row where that fills the GPU (24 warps an SM), else more, up
+    // to one for each group of heads. (A row's table entries and weights cost
+    // as much as a few of its heads: with 2 or 4 warps a row, 4096 rows took
+    // 26 and 34 us where one a row took 23.)
+    const int per = 32 / lph, groups = (a.n_q + per - 1) / per + (a.row_slot ? 2 * ((a.n_kv + per - 1) / per) : 0);
+    const long long want = (3552 + a.rows - 1) / a.rows;
     a.per_row = (int)(want < groups ? want : groups);
     const long long blocks = ((long long)a.rows * a.per_row + kWarps - 1) / kWarps;
     return launch_pdl(kernel, dim3((unsigned)blocks), dim3(kWarps * 32), 0, st, a);
@@ -194,13 +232,17 @@ cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
   // runs of 8 where the halves of what rotates and of what does not are whole
   // numbers of them
   if (a.rot % 16 == 0 && (a.hd - a.rot) % 16 == 0) {
-    if (a.hd <= 64) return go(qk_norm_rope_kernel<TI, TO, 8, 4>, 4);
-    if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 8, 8>, 8);
-    return go(qk_norm_rope_kernel<TI, TO, 8, 16>, 16);
+    if (a.rot == a.hd) {
+      if (a.hd == 64) return go(qk_norm_rope_kernel<TI, TO, 8, 4, true>, 4);
+      if (a.hd == 128) return go(qk_norm_rope_kernel<TI, TO, 8, 8, true>, 8);
+      if (a.hd == 256) return go(qk_norm_rope_kernel<TI, TO, 8, 16, true>, 16);
+    }
+    if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 8, 8, false>, 8);
+    return go(qk_norm_rope_kernel<TI, TO, 8, 16, false>, 16);
   }
-  if (a.hd <= 64) return go(qk_norm_rope_kernel<TI, TO, 4, 8>, 8);
-  if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 4, 16>, 16);
-  return go(qk_norm_rope_kernel<TI, TO, 4, 32>, 32);
+  if (a.hd <= 64) return go(qk_norm_rope_kernel<TI, TO, 4, 8, false>, 8);
+  if (a.hd <= 128) return go(qk_norm_rope_kernel<TI, TO, 4, 16, false>, 16);
+  return go(qk_norm_rope_kernel<TI, TO, 4, 32, false>, 32);
 }
 
 // whether the row-strided ranges [p, p + ((rows-1) ld + n) es) of two

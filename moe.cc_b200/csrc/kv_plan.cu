@@ -208,7 +208,7 @@ extern "C" int moe_kv_plan_dev(const int* past_len, const int* new_len, int n_se
   const int work = n_seq > row_cap ? n_seq : row_cap, each = kMaxThreads * (a.quads ? 4 : 1);
   const int threads = work <= 256 ? 256 : kMaxThreads;
   const int ctas = work <= 2 * kMaxThreads ? 1 : work / each < 148 ? (work + each - 1) / each : 148;
-  const bool in_place = ctas > 1 && ((kv_len && kv_len == past_len) || (free_head_out && free_head_out == free_head));
+  const bool in_place = ctas > 1 && ((kv_len && (kv_len == past_len || kv_len == new_len)) || (free_head_out && free_head_out == free_head));
   const size_t smem = sizeof(int) * 3 * (size_t)n_seq;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -68,11 +68,24 @@ template <> __device__ __forceinline__ float logit<float>(const void* x, long lo
 template <> __device__ __forceinline__ float logit<__nv_bfloat16>(const void* x, long long i) { return __bfloat162float(((const __nv_bfloat16*)x)[i]); }
 template <> __device__ __forceinline__ float logit<__half>(const void* x, long long i) { return __half2float(((const __half*)x)[i]); }
 
-// exp(x - top) with x = top = +inf counted as 1, and the sigmoid, in the type of the ranking
+// exp(x - top) with x = top = +inf counted as 1, and the sigmoid: for the
+// weights, in 64 bits, and (fast_) for the fp32 ranking, by the hardware's base-2
+// exponential (2^-22) and reciprocal (1 ulp).
 __device__ __forceinline__ float soft(float x, float top) { return x == top ? 1.0f : expf(x - top); }
 __device__ __forceinline__ float sigm(float x) { return 1.0f / (1.0f + expf(-x)); }
 __device__ __forceinline__ double soft64(float x, float top) { return x == top ? 1.0 : exp((double)x - (double)top); }
 __device__ __forceinline__ double sigm64(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_soft(float x, float top) { return x == top ? 1.0f : ex2((x - top) * 1.4426950408889634f); }
+__device__ __forceinline__ float fast_sigm(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(x * -1.4426950408889634f)));
+  return r;
+}
 
 // Scores plus bias of a lane's experts, in F; -inf for an expert that may not
 // be chosen (a NaN or -inf logit or bias).
@@ -83,7 +96,7 @@ __device__ __forceinline__ void choices(const RouteArgs& a, const float (&x)[EPL
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     if constexpr (sizeof(F) == 8) c[j] = a.softmax ? soft64(x[j], top) : sigm64(x[j]);
-    else c[j] = a.softmax ? soft(x[j], top) : sigm(x[j]);
+    else c[j] = a.softmax ? fast_soft(x[j], top) : fast_sigm(x[j]);
     if (!(x[j] > -INFINITY)) c[j] = 0;
     sum += c[j];
   }
@@ -106,22 +119,23 @@ __device__ __forceinline__ void choices(const RouteArgs& a, const float (&x)[EPL
 }
 
 // How far apart two fp32 choices must be for the exact ones to be ordered
-// alike. In units of 2^-24: a sigmoid errs by 4 (expf by 2 ulp, damped by
-// e^-x s < 1, sum and quotient), with the bias by |c| more, two of them by less
-// than 2^4 (1 + |u| + |v|); a softmax score relatively by |z| (its rounded
-// argument z = x - max; |z| s < 0.4), 4 (expf), 2 (quotient and product) and by
-// its sum, up to 37 roundings and the mean of |z|, below ln 1024 + 1: less than
-// 2^6, two of them and the bias 2^7 (1 + |u| + |v|). `drop`: the low bits of
-// either that were taken out, relatively 2^(drop - 23).
+// alike. In units of 2^-24: a sigmoid errs by 6 (the exponential by 4 and its
+// argument's rounding, both damped by e^-x s^2 < 1/4 and |x| e^-x s^2 < 1/2; the
+// sum by 1, the reciprocal by 2), with the bias by |c| more, two of them by less
+// than 2^4 (1 + |u| + |v|); a softmax score relatively by 2 |z| (its argument
+// z = x - max, rounded twice; |z| s < 0.4), 4 (the exponential), 2 (quotient and
+// product) and by its sum, up to 37 roundings, 4 and twice the mean of |z|,
+// below ln 1024 + 1: less than 2^6, two of them and the bias 2^7 (1 + |u| + |v|).
+// `drop`: the low bits of either that were taken out, relatively 2^(drop - 23).
 __device__ __forceinline__ float margin(const RouteArgs& a, float u, float v, float drop) {
   const float m = fabsf(u) + fabsf(v);
   return fmaf(m, drop, (a.softmax ? 0x1p-17f : 0x1p-20f) * (1.0f + m));
 }
 
-// Takes the experts outside the `keep` best groups out of c. cut[0], cut[1]:
-// the least sum that stays and the largest that does not.
+// Which of the groups stay, a bit at lane (group * lanes_per_group). cut[0],
+// cut[1]: the least sum that stays and the largest that does not.
 template <typename F, int EPL>
-__device__ __forceinline__ void keep_groups(const RouteArgs& a, F* mine, F (&c)[EPL], F (&cut)[2]) {
+__device__ __forceinline__ unsigned best_groups(const RouteArgs& a, F* mine, const F (&c)[EPL], F (&cut)[2]) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
 #pragma unroll
@@ -149,14 +163,51 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, F* mine, F (&c)[
     before += v > gs || (v == gs && h < grp);
   }
   const bool head = grp < a.groups && lane % lpg == 0;
-  const unsigned stays = __ballot_sync(~0u, head && before < a.keep);
   cut[0] = __shfl_sync(~0u, gs, __ffs(__ballot_sync(~0u, head && before == a.keep - 1)) - 1);
   cut[1] = __shfl_sync(~0u, gs, __ffs(__ballot_sync(~0u, head && before == a.keep)) - 1);
+  return __ballot_sync(~0u, head && before < a.keep);
+}
+
+// The same by choices in 64 bits.
+template <int EPL>
+__device__ __noinline__ unsigned best_groups64(const RouteArgs& a, const float (&x)[EPL], float top, double* mine) {
+  double c[EPL], cut[2];
+  choices<double, EPL>(a, x, top, c);
+  return best_groups<double, EPL>(a, mine, c, cut);
+}
+
+// Whether expert j * 32 + lane is in a group that stays.
+__device__ __forceinline__ bool stays_in(const RouteArgs& a, unsigned stays, int j) {
+  const int e = j * 32 + (threadIdx.x & 31);
+  return e >= a.E || (stays >> ((int)a.group.div((unsigned)e) * a.lanes_per_group)) & 1;
+}
+
+// Keys of a lane, the largest first (odd-even exchange; EPL is a power of two).
+template <int EPL>
+__device__ __forceinline__ void sort_keys(unsigned (&k)[EPL]) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = j * 32 + lane, ge = (int)a.group.div((unsigned)e);
-    if (e < a.E && !((stays >> (ge * lpg)) & 1)) c[j] = -INFINITY;
-  }
+  for (int p = 1; p < EPL; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < EPL; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (j + i + q < EPL && (j + i) / (2 * p) == (j + i + q) / (2 * p)) {
+            const unsigned u = k[j + i], v = k[j + i + q];
+            k[j + i] = max(u, v);
+            k[j + i + q] = min(u, v);
+          }
+}
+// One round over sorted unique keys: the largest of the warp leaves its lane.
+template <int EPL>
+__device__ __forceinline__ unsigned pop(unsigned (&k)[EPL]) {
+  const unsigned best = __reduce_max_sync(~0u, k[0]);
+  const bool own = k[0] == best;
+#pragma unroll
+  for (int j = 0; j + 1 < EPL; ++j) k[j] = own ? k[j + 1] : k[j];
+  if (own) k[EPL - 1] = 0u;
+  return best;
 }
 
 // One round: the largest of the warp's keys, the lowest expert that has it
@@ -198,16 +249,13 @@ __device__ __forceinline__ int take(unsigned long long (&key)[EPL]) {
 
 // The token's choice ranked in 64 bits; lane r returns the r-th.
 template <int EPL>
-__device__ __noinline__ int choose64(const RouteArgs& a, const float (&x)[EPL], float top, double* mine) {
+__device__ __noinline__ int choose64(const RouteArgs& a, const float (&x)[EPL], float top, unsigned stays) {
   double c[EPL];
   unsigned long long key[EPL];
   choices<double, EPL>(a, x, top, c);
-  if (a.groups > 1) {
-    double cut[2];
-    keep_groups<double, EPL>(a, mine, c, cut);
-  }
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) key[j] = c[j] > -INFINITY ? key_of(c[j]) : 0ull;
+  for (int j = 0; j < EPL; ++j)
+    key[j] = c[j] > -INFINITY && (a.groups == 1 || stays_in(a, stays, j)) ? key_of(c[j]) : 0ull;
   int chosen = -1;
   for (int r = 0; r < a.topk; ++r) {
     const int e = take<EPL>(key);
@@ -273,39 +321,57 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
     for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
     const unsigned tk = __reduce_max_sync(~0u, key_of(top));
     top = value_of(tk);
-    float c[EPL], cut[2] = {INFINITY, -INFINITY};
+    float c[EPL];
     choices<float, EPL>(a, x, top, c);
-    if (a.groups > 1) keep_groups<float, EPL>(a, (float*)(choice_sm + warp * (EPL * 32)), c, cut);
+    unsigned stays = ~0u;
+    if (a.groups > 1) {
+      double* mine = choice_sm + warp * (EPL * 32);
+      float cut[2];
+      stays = best_groups<float, EPL>(a, (float*)mine, c, cut);
+      if (cut[0] - cut[1] < 2 * margin(a, cut[0], cut[1], 0.f)) stays = best_groups64<EPL>(a, x, top, mine);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (!stays_in(a, stays, j)) c[j] = -INFINITY;
+    }
     // Keys: the fp32 choice without its lowest bits, which hold the index from
-    // the top down. The list runs on past top_k until the next one is clearly
-    // behind; then nothing outside it can belong in it.
+    // the top down. Lane n keeps the n-th; top_k + 1 of them, and on until the
+    // next one is clearly behind the one before: nothing outside the list can
+    // then belong in its first top_k.
     constexpr unsigned kLow = EPL * 32 - 1;
     constexpr float kDrop = (float)(EPL * 32) * 0x1p-23f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j)
       key[j] = c[j] > -INFINITY ? (key_of(c[j]) & ~kLow) | (kLow - (j * 32 + lane)) : 0u;
-    float last = INFINITY;
+    sort_keys<EPL>(key);
+    unsigned mine = 0u;
     int n = 0;
-    bool unsure = false, anew = a.groups > 1 && cut[0] - cut[1] < 2 * margin(a, cut[0], cut[1], 0.f);
-    for (;;) {
-      unsigned best = key[0];
-#pragma unroll
-      for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
-      best = __reduce_max_sync(~0u, best);
+    for (; n < min(a.topk + 1, 32); ++n) {
+      const unsigned best = pop<EPL>(key);
       if (best == 0u) break;
-      const float v = value_of(best & ~kLow);
-      const bool near = !(last - v >= margin(a, last, v, kDrop));
-      if (n >= a.topk && !near) break;
-      unsure |= near;
-      if (n == 32) { anew = true; break; }
-      if (lane == n) chosen = (int)(kLow - (best & kLow));
-      ++n;
-      last = v;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) key[j] = key[j] == best ? 0u : key[j];
+      if (lane == n) mine = best;
     }
-    if (anew) chosen = choose64<EPL>(a, x, top, choice_sm + warp * (EPL * 32));
-    else if (unsure) chosen = order64<T, EPL>(a, x, top, t, chosen, n);
+    auto near = [&]() -> unsigned {                        // bit i: entry i + 1 is not clearly behind entry i
+      const float u = value_of(mine & ~kLow), v = __shfl_down_sync(~0u, u, 1);
+      return __ballot_sync(~0u, lane + 1 < n && !(u - v >= margin(a, u, v, kDrop)));
+    };
+    unsigned close = near();
+    bool anew = false;
+    while (n > a.topk && (close >> (n - 2)) & 1) {         // the last is not: the list goes on
+      const unsigned best = pop<EPL>(key);
+      if (best == 0u) break;
+      if (n == 32) { anew = true; break; }
+      if (lane == n) mine = best;
+      ++n;
+      close = near();
+    }
+    if (a.topk == 32 && !anew) {                           // no lane is left to look behind the last
+      const unsigned best = pop<EPL>(key);
+      const float u = __shfl_sync(~0u, value_of(mine & ~kLow), 31), v = value_of(best & ~kLow);
+      anew = best != 0u && !(u - v >= margin(a, u, v, kDrop));
+    }
+    chosen = mine ? (int)(kLow - (mine & kLow)) : -1;
+    if (anew) chosen = choose64<EPL>(a, x, top, stays);
+    else if (close) chosen = order64<T, EPL>(a, x, top, t, chosen, __popc(__ballot_sync(~0u, mine != 0u)));
     if (lane >= a.topk) chosen = -1;
   } else if constexpr (sizeof(T) == 2) {
     // the logit's 16 bits above, the index from the top down below them
@@ -318,16 +384,14 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
       b = (b ^ (b >> 15 ? 0xffffu : 0x8000u)) & 0xffffu;
       key[j] = x[j] > -INFINITY ? b << 16 | (0xffffu - e) : 0u;
     }
+    sort_keys<EPL>(key);
+    unsigned mine = 0u;
     for (int r = 0; r < a.topk; ++r) {
-      unsigned best = key[0];
-#pragma unroll
-      for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
-      best = __reduce_max_sync(~0u, best);
+      const unsigned best = pop<EPL>(key);
       if (best == 0u) break;
-      if (lane == r) chosen = 0xffff - (int)(best & 0xffffu);
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) key[j] = key[j] == best ? 0u : key[j];
+      if (lane == r) mine = best;
     }
+    chosen = mine ? 0xffff - (int)(mine & 0xffffu) : -1;
   } else {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) key[j] = x[j] > -INFINITY ? key_of(x[j]) : 0u;

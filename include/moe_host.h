@@ -122,8 +122,21 @@ int mh_advance(MhModel* m, int T);
 int mh_ep_setup(MhModel* m, int max_rows_per_call, void* handle_out);
 int mh_ep_connect(MhModel* m, const void* handles);
 
+/* Moves the KV caches, and the attention over them, to the GPU: the caches
+ * become pages of page_size positions in device memory (`dtype` MOE_DTYPE_F32,
+ * _F16 or _BF16), and mh_attention hands the projected rows to
+ * moe_qk_norm_rope_dev and moe_paged_attention_dev, with the projections, norms
+ * and the output product on the CPU as before. Same rotation angles as the CPU
+ * path (fp32 position * inverse frequency). The attention's sums run in another
+ * order and, with 16 bits, over rounded queries, keys and values, so logits are
+ * close to the CPU path's but not equal bit for bit. Before the first tokens
+ * (position 0); frees the host caches. head_dim a multiple of 8 up to 256
+ * (MOE_ERR_UNSUPPORTED otherwise). The device current at the call is used. */
+int mh_kv_device(MhModel* m, int dtype, int page_size);
+
 /* Accumulated wall time of the MoE calls per layer since the last reset
- * (ms[n_layers], calls[n_layers]; either may be NULL) and of the CPU part. */
+ * (ms[n_layers], calls[n_layers]; either may be NULL) and of the CPU part
+ * (with mh_kv_device its time includes the attention on the GPU). */
 int mh_timing(const MhModel* m, double* moe_ms, long* moe_calls, double* cpu_ms);
 void mh_timing_reset(MhModel* m);
 

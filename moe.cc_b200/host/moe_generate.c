@@ -6,6 +6,7 @@
  *   moe_generate [--bin FILE] [--layers 48] [--dtype q8|q4] [--batch 1]
  *                [--prompt 64] [--steps 256] [--ctx 4096] [--kv-fill 0]
  *                [--seed 1] [--device 0] [--ep-dir DIR] [--out FILE]
+ *                [--kv host|f32|f16|bf16] [--page 16]
  *
  * Without --bin the model is the Qwen3-30B-A3B shape with random-init
  * weights (mh_synth: fp32 ~ N(0, 0.02), experts quantised on the GPU,
@@ -15,6 +16,10 @@
  * Prints one JSON line: decode tokens/s over all sequences, the prefill time,
  * and the MoE wall time per layer call (host-pointer moe_ffn, copies
  * included) against the host attention time.
+ *
+ * --kv f32|f16|bf16 keeps the KV caches, and the attention over them, on the GPU
+ * in pages of --page positions (mh_kv_device); "host_ms_per_step" then includes
+ * that attention.
  *
  * Expert parallelism: started as WORLD_SIZE processes (RANK, LOCAL_RANK in
  * the environment, e.g. by torchrun) with --ep-dir naming a directory all of
@@ -80,6 +85,8 @@ int main(int argc, char** argv) {
   const char* ep_dir = NULL;
   const char* out_path = NULL;    /* --out FILE: this rank's tokens to FILE.<rank> */
   int layers = 48, dtype = MOE_DTYPE_Q8, batch = 1, prompt = 64, steps = 256, ctx = 4096, kv_fill = 0, device = 0;
+  const char* kv = "host";
+  int page = 16;
   unsigned long long seed = 1;
   for (int i = 1; i < argc; ++i) {
     const char* a = argv[i];
@@ -97,6 +104,8 @@ int main(int argc, char** argv) {
     else if (!strcmp(a, "--device")) device = atoi(v);
     else if (!strcmp(a, "--ep-dir")) ep_dir = v;
     else if (!strcmp(a, "--out")) out_path = v;
+    else if (!strcmp(a, "--kv")) kv = v;
+    else if (!strcmp(a, "--page")) page = atoi(v);
     else { fprintf(stderr, "unknown option %s\n", a); return 2; }
     ++i;
   }
@@ -129,6 +138,10 @@ int main(int argc, char** argv) {
   const double t_load = now_ms();
   MhModel* m = mh_create(&cfg, batch, ctx, 0);
   if (!m) { fprintf(stderr, "%s\n", mh_last_error()); return 1; }
+  if (strcmp(kv, "host")) {
+    const int kd = !strcmp(kv, "f32") ? MOE_DTYPE_F32 : !strcmp(kv, "f16") ? MOE_DTYPE_F16 : !strcmp(kv, "bf16") ? MOE_DTYPE_BF16 : -1;
+    if (mh_kv_device(m, kd, page) != MOE_OK) { fprintf(stderr, "--kv %s: %s\n", kv, mh_last_error()); mh_free(m); return 1; }
+  }
   int rc = bin ? mh_load_bin(m, bin) : mh_synth(m, seed, dtype, 0.02f);
   if (rc) { fprintf(stderr, "weights: %s\n", mh_last_error()); mh_free(m); return 1; }
   const double load_ms = now_ms() - t_load;
@@ -209,12 +222,12 @@ int main(int argc, char** argv) {
   const int dsteps = steps - 1;
   if (rank == 0)
   printf("{\"workload\": \"greedy decode\", \"source\": \"%s\", \"layers\": %d, \"dtype\": \"%s\", "
-         "\"ep_world\": %d, \"batch\": %d, \"prompt\": %d, \"steps\": %d, \"kv_fill\": %d, \"load_s\": %.2f, "
+         "\"ep_world\": %d, \"batch\": %d, \"prompt\": %d, \"steps\": %d, \"kv_fill\": %d, \"kv\": \"%s\", \"load_s\": %.2f, "
          "\"prefill_ms\": %.2f, \"decode_tok_s\": %.3f, \"decode_ms_per_step\": %.3f, "
          "\"moe_ms_per_layer_call\": %.4f, \"moe_ms_per_step\": %.3f, \"host_ms_per_step\": %.3f, "
          "\"first_tokens\": [%d, %d, %d, %d]}\n",
          bin ? "bin" : "synthetic", cfg.n_layers, dtype == MOE_DTYPE_Q8 ? "q8" : "q4", world, batch * world, prompt,
-         steps, kv_fill, load_ms / 1e3, prefill_ms,
+         steps, kv_fill, kv, load_ms / 1e3, prefill_ms,
          dsteps > 0 ? (double)batch * world * dsteps / (decode_ms / 1e3) : 0.0,
          dsteps > 0 ? decode_ms / dsteps : 0.0, call_total ? moe_total / call_total : 0.0,
          dsteps > 0 ? moe_total / dsteps : 0.0, dsteps > 0 ? cpu_ms / dsteps : 0.0,

@@ -66,6 +66,20 @@ struct MhModel {
   int ep_on, ep_cap;
   float *d_xn, *d_xo;
   cudaStream_t ep_stream;
+  /* device KV (mh_kv_device): paged caches of every layer, page (j, b) = j*batch
+     + b of a layer for pages j of sequence b; the plan of the rows at
+     (plan_pos, plan_T); staging of the projected rows */
+  int kv_dtype, kv_page, kv_max_pages, plan_pos, plan_T, plan_cap, kv_cap;
+  int kv_on;
+  void *d_kc, *d_vc;
+  float* d_rope;                 /* [max_ctx][head_dim]: cosines, sines */
+  int *d_table, *d_free, *d_len, *d_rows;
+  float* h_qkv;                  /* page-locked [q | k | v | q_norm | k_norm] */
+  float* d_qkv;
+  void *d_q, *d_out, *h_out;
+  void* d_ws;
+  size_t ws_bytes;
+  cudaStream_t kv_stream;
 };
 
 static _Thread_local char g_err[512];   /* per calling thread */
@@ -359,8 +373,31 @@ static void free_scratch(MhModel* m) {
   m->cap_rows = 0;
 }
 
+static void free_kv_rows(MhModel* m) {
+  cudaFreeHost(m->h_qkv); cudaFreeHost(m->h_out);
+  cudaFree(m->d_qkv); cudaFree(m->d_q); cudaFree(m->d_out);
+  m->h_qkv = m->d_qkv = NULL;
+  m->h_out = m->d_q = m->d_out = NULL;
+  m->kv_cap = 0;
+}
+
+static void free_kv(MhModel* m) {
+  free_kv_rows(m);
+  cudaFree(m->d_kc); cudaFree(m->d_vc); cudaFree(m->d_rope); cudaFree(m->d_table); cudaFree(m->d_free);
+  cudaFree(m->d_len); cudaFree(m->d_ws); cudaFree(m->d_rows);
+  if (m->kv_stream) cudaStreamDestroy(m->kv_stream);
+  m->d_kc = m->d_vc = m->d_ws = NULL;
+  m->d_rope = NULL;
+  m->d_table = m->d_free = m->d_len = m->d_rows = NULL;
+  m->plan_cap = m->plan_T = 0;
+  m->kv_stream = NULL;
+  m->ws_bytes = 0;
+  m->kv_on = 0;
+}
+
 void mh_free(MhModel* m) {
   if (!m) return;
+  if (m->kv_on) free_kv(m);
   if (m->d_xn) cudaFree(m->d_xn);
   if (m->d_xo) cudaFree(m->d_xo);
   if (m->ep_stream) cudaStreamDestroy(m->ep_stream);
@@ -438,6 +475,183 @@ static float* kv_row(const MhModel* m, float* base, int layer, int b, int p) {
   return base + (((size_t)layer * m->batch + b) * m->max_ctx + p) * m->Dkv;
 }
 
+/* ---- attention on the GPU over paged caches (mh_kv_device) ------------------ */
+
+static size_t kv_elem(int dtype) { return dtype == MOE_DTYPE_F32 ? 4 : 2; }
+
+static float half_bits(unsigned h) {
+  const unsigned s = (h & 0x8000u) << 16, e = (h >> 10) & 31u, f = h & 0x3ffu;
+  unsigned u;
+  float v;
+  if (e == 0) { v = (float)f * 0x1p-24f; memcpy(&u, &v, 4); u |= s; }
+  else u = e == 31 ? s | 0x7f800000u | (f << 13) : s | ((e + 112u) << 23) | (f << 13);
+  memcpy(&v, &u, 4);
+  return v;
+}
+
+#define KV_OK(call, what)                                                                        \
+  do {                                                                                           \
+    cudaError_t e_ = (call);                                                                     \
+    if (e_ != cudaSuccess) return fail(e_ == cudaErrorMemoryAllocation ? MOE_ERR_NOMEM : MOE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e_)); \
+  } while (0)
+
+static MoeKvCache kv_layer(const MhModel* m, int layer) {
+  const int hd = m->c.head_dim, n_pages = m->batch * m->kv_max_pages;
+  const size_t layer_bytes = (size_t)n_pages * m->kv_page * m->Dkv * kv_elem(m->kv_dtype);
+  MoeKvCache c = {(char*)m->d_kc + layer * layer_bytes, (char*)m->d_vc + layer * layer_bytes, m->kv_dtype, n_pages,
+                  m->kv_page, m->c.n_kv, hd, (long long)m->kv_page * m->Dkv, m->Dkv, hd};
+  return c;
+}
+
+static int kv_rows(MhModel* m, int R) {
+  if (R <= m->kv_cap) return MOE_OK;
+  free_kv_rows(m);
+  const size_t es = kv_elem(m->kv_dtype), wide = (size_t)R * (m->Dq + 2 * (size_t)m->Dkv) + 2 * (size_t)m->c.head_dim;
+  KV_OK(cudaHostAlloc((void**)&m->h_qkv, sizeof(float) * wide, cudaHostAllocDefault), "attention rows");
+  KV_OK(cudaHostAlloc(&m->h_out, es * (size_t)R * m->Dq, cudaHostAllocDefault), "attention rows");
+  KV_OK(cudaMalloc((void**)&m->d_qkv, sizeof(float) * wide), "attention rows");
+  KV_OK(cudaMalloc(&m->d_q, es * (size_t)R * m->Dq), "attention rows");
+  KV_OK(cudaMalloc(&m->d_out, es * (size_t)R * m->Dq), "attention rows");
+  m->kv_cap = R;
+  return MOE_OK;
+}
+
+/* Pages and rows of T new tokens a sequence at position pos. The free list of
+   the call is the pages that the sequences get, in its order (sequence after
+   sequence), so page j of a sequence is the same whatever steps led to it. */
+static int kv_plan(MhModel* m, int pos, int T) {
+  if (m->plan_T == T && m->plan_pos == pos) return MOE_OK;
+  const int B = m->batch, ps = m->kv_page, cap = B * T;
+  if (cap > m->plan_cap) {
+    cudaFree(m->d_rows);           /* waits for what still reads it */
+    m->d_rows = NULL;
+    m->plan_cap = m->plan_T = 0;
+    KV_OK(cudaMalloc((void**)&m->d_rows, sizeof(int) * 3 * (size_t)cap), "attention plan");
+    m->plan_cap = cap;
+  }
+  m->plan_T = 0;                   /* none, should the calls below fail */
+  const int held = (pos + ps - 1) / ps, need = (pos + T + ps - 1) / ps, n = (need - held) * B;
+  int* h = (int*)malloc(sizeof(int) * ((size_t)n + 2 * (size_t)B));
+  if (!h) return fail(MOE_ERR_NOMEM, "attention plan");
+  for (int b = 0, i = 0; b < B; ++b) {
+    for (int j = held; j < need; ++j) h[2 * B + i++] = j * B + b;
+    h[b] = pos;
+    h[B + b] = T;
+  }
+  /* pageable memory: the copies have left h when the calls return */
+  cudaError_t e = cudaMemcpyAsync(m->d_len, h, sizeof(int) * 2 * (size_t)B, cudaMemcpyHostToDevice, m->kv_stream);
+  if (e == cudaSuccess && n) e = cudaMemcpyAsync(m->d_free, h + 2 * B, sizeof(int) * (size_t)n, cudaMemcpyHostToDevice, m->kv_stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(m->kv_stream);
+  free(h);
+  KV_OK(e, "attention plan");
+  int* r = m->d_rows;
+  const int rc = moe_kv_plan_dev(m->d_len, m->d_len + B, B, ps, B * m->kv_max_pages, m->d_free, n, NULL, m->d_table,
+                                 m->kv_max_pages, NULL, r, r + m->plan_cap, r + 2 * (size_t)m->plan_cap, cap, NULL, NULL,
+                                 m->kv_stream);
+  if (rc) return fail(rc, "%s", moe_cuda_last_error());
+  m->plan_pos = pos;
+  m->plan_T = T;
+  return MOE_OK;
+}
+
+/* q, k, v of the new rows (in h_qkv) -> norm, rotation, append, attention ->
+   m->hcat, for layer l at the current position. */
+static int kv_attention(MhModel* m, int l, int T) {
+  const int R = m->batch * T, hd = m->c.head_dim, nq = m->c.n_q;
+  const MhLayerWeights* w = &m->layers[l].w;
+  const size_t rows = (size_t)R * (m->Dq + 2 * (size_t)m->Dkv);
+  float *qn = m->h_qkv + rows, *kn = qn + hd;
+  if (w->q_norm) memcpy(qn, w->q_norm, sizeof(float) * (size_t)hd);
+  if (w->k_norm) memcpy(kn, w->k_norm, sizeof(float) * (size_t)hd);
+  int rc = kv_plan(m, m->pos, T);
+  if (rc) return rc;
+  KV_OK(cudaMemcpyAsync(m->d_qkv, m->h_qkv, sizeof(float) * (rows + 2 * (size_t)hd), cudaMemcpyHostToDevice, m->kv_stream),
+        "attention rows to the device");
+  const MoeKvCache c = kv_layer(m, l);
+  const float *dq = m->d_qkv, *dk = dq + (size_t)R * m->Dq, *dv = dk + (size_t)R * m->Dkv, *dqn = dq + rows;
+  const int *seq = m->d_rows, *pos = seq + m->plan_cap, *slot = pos + m->plan_cap;
+  if ((rc = moe_qk_norm_rope_dev(dq, m->Dq, dk, m->Dkv, dv, m->Dkv, MOE_DTYPE_F32, R, nq, w->q_norm ? dqn : NULL,
+                                 w->k_norm ? dqn + hd : NULL, m->c.rms_eps, m->d_rope, hd, m->max_ctx, pos, slot, m->d_q,
+                                 m->Dq, &c, m->kv_stream)))
+    return fail(rc, "%s", moe_cuda_last_error());
+  const int max_kv = m->pos + T;
+  const size_t need = moe_paged_attention_workspace(R, nq, &c, max_kv);
+  if (need > m->ws_bytes) {
+    KV_OK(cudaStreamSynchronize(m->kv_stream), "attention workspace");
+    cudaFree(m->d_ws);
+    m->d_ws = NULL;
+    m->ws_bytes = 0;
+    KV_OK(cudaMalloc(&m->d_ws, need), "attention workspace");
+    m->ws_bytes = need;
+  }
+  if ((rc = moe_paged_attention_dev(m->d_q, m->Dq, &c, m->d_table, m->batch, m->kv_max_pages, seq, pos, R, nq, max_kv,
+                                    1.0f / sqrtf((float)hd), m->d_out, m->Dq, NULL, m->d_ws, m->ws_bytes, m->kv_stream)))
+    return fail(rc, "%s", moe_cuda_last_error());
+  const size_t n = (size_t)R * m->Dq;
+  KV_OK(cudaMemcpyAsync(m->h_out, m->d_out, n * kv_elem(m->kv_dtype), cudaMemcpyDeviceToHost, m->kv_stream),
+        "attention rows from the device");
+  KV_OK(cudaStreamSynchronize(m->kv_stream), "attention");
+  if (m->kv_dtype == MOE_DTYPE_F32) memcpy(m->hcat, m->h_out, sizeof(float) * n);
+  else {
+    const unsigned short* h = (const unsigned short*)m->h_out;
+    const int bf = m->kv_dtype == MOE_DTYPE_BF16;
+    for (size_t i = 0; i < n; ++i) {
+      if (bf) { const unsigned u = (unsigned)h[i] << 16; memcpy(m->hcat + i, &u, 4); }
+      else m->hcat[i] = half_bits(h[i]);
+    }
+  }
+  return MOE_OK;
+}
+
+int mh_kv_device(MhModel* m, int dtype, int page_size) {
+  if (!m || page_size < 1 || (dtype != MOE_DTYPE_F32 && dtype != MOE_DTYPE_F16 && dtype != MOE_DTYPE_BF16))
+    return fail(MOE_ERR_INVALID, "mh_kv_device: bad argument");
+  if (m->pos != 0) return fail(MOE_ERR_INVALID, "mh_kv_device: the model already holds %d positions", m->pos);
+  const int hd = m->c.head_dim, d2 = hd / 2;
+  if (hd % 8 || hd > 256) return fail(MOE_ERR_UNSUPPORTED, "mh_kv_device: head_dim %d (multiples of 8 up to 256)", hd);
+  const long long max_pages = ((long long)m->max_ctx + page_size - 1) / page_size;
+  if (max_pages * m->batch * page_size > 0x7fffffffll)
+    return fail(MOE_ERR_UNSUPPORTED, "mh_kv_device: more than 2^31 - 1 positions a layer");
+  if (m->kv_on) free_kv(m);
+  m->kv_on = 1;                    /* what is allocated below goes with the model */
+  m->kv_dtype = dtype;
+  m->kv_page = page_size;
+  m->kv_max_pages = (int)max_pages;
+  m->plan_T = 0;
+  const size_t bytes = (size_t)m->c.n_layers * m->batch * m->kv_max_pages * page_size * m->Dkv * kv_elem(dtype);
+  const size_t entries = (size_t)m->batch * m->kv_max_pages;
+  float* rope = (float*)malloc(sizeof(float) * (size_t)m->max_ctx * hd);
+  int rc = MOE_OK;
+  cudaError_t e;
+  if (!rope) rc = fail(MOE_ERR_NOMEM, "mh_kv_device: host memory");
+  for (int p = 0; !rc && p < m->max_ctx; ++p)
+    for (int i = 0; i < d2; ++i) {
+      const float a = (float)p * m->inv_freq[i];
+      rope[(size_t)p * hd + i] = cosf(a);
+      rope[(size_t)p * hd + d2 + i] = sinf(a);
+    }
+  if (!rc && ((e = cudaMalloc(&m->d_kc, bytes)) || (e = cudaMalloc(&m->d_vc, bytes)) ||
+              (e = cudaMalloc((void**)&m->d_rope, sizeof(float) * (size_t)m->max_ctx * hd)) ||
+              (e = cudaMalloc((void**)&m->d_table, sizeof(int) * entries)) ||
+              (e = cudaMalloc((void**)&m->d_free, sizeof(int) * entries)) ||
+              (e = cudaMalloc((void**)&m->d_len, sizeof(int) * 2 * (size_t)m->batch)) ||
+              (e = cudaStreamCreateWithFlags(&m->kv_stream, cudaStreamNonBlocking)) ||
+              (e = cudaMemset(m->d_table, 0xff, sizeof(int) * entries)) ||
+              (e = cudaMemcpy(m->d_rope, rope, sizeof(float) * (size_t)m->max_ctx * hd, cudaMemcpyHostToDevice))))
+    rc = fail(e == cudaErrorMemoryAllocation ? MOE_ERR_NOMEM : MOE_ERR_CUDA, "mh_kv_device (2 x %zu bytes of cache): %s", bytes,
+              cudaGetErrorString(e));
+  free(rope);
+  if (rc) {
+    cudaGetLastError();
+    free_kv(m);
+    return rc;
+  }
+  free(m->kc);
+  free(m->vc);
+  m->kc = m->vc = NULL;
+  return MOE_OK;
+}
+
 int mh_attention(MhModel* m, int layer, const float* x, int T, float* x_after, float* x_norm2) {
   if (!m || layer < 0 || layer >= m->c.n_layers || !x || !x_after || !x_norm2 || T < 1)
     return fail(MOE_ERR_INVALID, "mh_attention: bad argument");
@@ -452,14 +666,23 @@ int mh_attention(MhModel* m, int layer, const float* x, int T, float* x_after, f
   if (rc) return rc;
   const double t0 = now_ms();
 
+  float *q = m->q, *k = m->k, *v = m->v;
+  if (m->kv_on) {                  /* straight into the page-locked staging */
+    if ((rc = kv_rows(m, R))) return rc;
+    q = m->h_qkv; k = q + (size_t)R * Dq; v = k + (size_t)R * Dkv;
+  }
   rmsnorm_rows(x, w->rms1_w, R, D, eps, m->xn1);
-  mm_f32(m->xn1, w->Wq, m->q, R, Dq, D);
-  mm_f32(m->xn1, w->Wk, m->k, R, Dkv, D);
-  mm_f32(m->xn1, w->Wv, m->v, R, Dkv, D);
+  mm_f32(m->xn1, w->Wq, q, R, Dq, D);
+  mm_f32(m->xn1, w->Wk, k, R, Dkv, D);
+  mm_f32(m->xn1, w->Wv, v, R, Dkv, D);
   for (int r = 0; r < R; ++r) {
-    if (w->bq) for (int i = 0; i < Dq; ++i) m->q[(size_t)r * Dq + i] += w->bq[i];
-    if (w->bk) for (int i = 0; i < Dkv; ++i) m->k[(size_t)r * Dkv + i] += w->bk[i];
-    if (w->bv) for (int i = 0; i < Dkv; ++i) m->v[(size_t)r * Dkv + i] += w->bv[i];
+    if (w->bq) for (int i = 0; i < Dq; ++i) q[(size_t)r * Dq + i] += w->bq[i];
+    if (w->bk) for (int i = 0; i < Dkv; ++i) k[(size_t)r * Dkv + i] += w->bk[i];
+    if (w->bv) for (int i = 0; i < Dkv; ++i) v[(size_t)r * Dkv + i] += w->bv[i];
+  }
+  if (m->kv_on) {
+    if ((rc = kv_attention(m, layer, T))) return rc;
+    goto out_product;
   }
 #pragma omp parallel for schedule(static)
   for (int r = 0; r < R; ++r) {
@@ -522,6 +745,7 @@ int mh_attention(MhModel* m, int layer, const float* x, int T, float* x_after, f
     }
   }
 
+out_product:
   mm_f32(m->hcat, w->Wo, m->ao, R, D, Dq);
   if (w->bo) for (int r = 0; r < R; ++r) for (int i = 0; i < D; ++i) m->ao[(size_t)r * D + i] += w->bo[i];
   for (size_t i = 0; i < (size_t)R * D; ++i) x_after[i] = x[i] + m->ao[i];
@@ -902,12 +1126,44 @@ out:
   return rc;
 }
 
+/* mh_fill_kv into the paged caches: the same streams, appended as they are. */
+static int kv_fill(MhModel* m, int ctx, uint64_t seed, float std) {
+  const size_t row = (size_t)ctx * m->Dkv;
+  float* tmp = NULL;
+  int rc = MOE_OK;
+  if ((long long)ctx * m->batch > 0x7fffffffll / 3) return fail(MOE_ERR_UNSUPPORTED, "mh_fill_kv: too many rows");
+  if ((rc = kv_plan(m, 0, ctx))) return rc;
+  const int* slot = m->d_rows + 2 * (size_t)m->plan_cap;
+  CUDA_OK(cudaStreamSynchronize(m->kv_stream), "attention plan");
+  CUDA_OK(cudaMalloc((void**)&tmp, 2 * sizeof(float) * row), "device staging");
+  for (int l = 0; l < m->c.n_layers; ++l) {
+    const MoeKvCache c = kv_layer(m, l);
+    for (int b = 0; b < m->batch; ++b) {
+      const uint64_t blk = ((uint64_t)l * m->batch + b) * 2;
+      if ((rc = moe_synth_normal_dev(stream_seed(seed, 65534, blk), 0, row, std, tmp, m->kv_stream)) ||
+          (rc = moe_synth_normal_dev(stream_seed(seed, 65534, blk + 1), 0, row, std, tmp + row, m->kv_stream)) ||
+          (rc = moe_qk_norm_rope_dev(NULL, 0, tmp, m->Dkv, tmp + row, m->Dkv, MOE_DTYPE_F32, ctx, 0, NULL, NULL, 0.f, NULL, 0,
+                                     0, NULL, slot + (size_t)b * ctx, NULL, 0, &c, m->kv_stream))) {
+        rc = fail(rc, "%s", moe_cuda_last_error());
+        goto out;
+      }
+    }
+  }
+  CUDA_OK(cudaStreamSynchronize(m->kv_stream), "attention caches");
+  m->pos = ctx;
+out:
+  cudaStreamSynchronize(m->kv_stream);
+  cudaFree(tmp);
+  return rc;
+}
+
 int mh_fill_kv(MhModel* m, int ctx, uint64_t seed, float std) {
   if (!m || ctx < 0 || ctx > m->max_ctx) return fail(MOE_ERR_INVALID, "mh_fill_kv: bad context");
   int rc = MOE_OK;
   const size_t row = (size_t)ctx * m->Dkv;           /* one (layer, sequence) block */
   float* tmp = NULL;
   if (row == 0) { m->pos = ctx; return MOE_OK; }
+  if (m->kv_on) return kv_fill(m, ctx, seed, std);
   CUDA_OK(cudaMalloc((void**)&tmp, sizeof(float) * row), "device staging");
   for (int l = 0; l < m->c.n_layers; ++l)
     for (int b = 0; b < m->batch; ++b)

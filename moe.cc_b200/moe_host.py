@@ -17,6 +17,7 @@ EXPORTS = (
     "mh_config_from_bin", "mh_load_bin", "mh_synth", "mh_pos", "mh_reset", "mh_fill_kv",
     "mh_step", "mh_generate", "mh_pick_greedy", "mh_embed", "mh_attention", "mh_moe",
     "mh_head", "mh_advance", "mh_timing", "mh_timing_reset", "mh_ep_setup", "mh_ep_connect",
+    "mh_kv_device",
 )
 # include/moe_model.h (model.c's call surface, served by the same library)
 MODEL_EXPORTS = ("layer_forward_f32", "model_forward_f32", "moe_model_release")
@@ -58,6 +59,7 @@ def lib():
             "mh_advance": ([vp, i], i), "mh_timing": ([vp, vp, vp, vp], i),
             "mh_timing_reset": ([vp], None),
             "mh_ep_setup": ([vp, i, vp], i), "mh_ep_connect": ([vp, vp], i),
+            "mh_kv_device": ([vp, i, i], i),
         }
         sig["layer_forward_f32"] = ([vp, i, i, vp, f] + [vp] * 10 + [i, i, i, i, f, vp, f, vp, vp] + [vp] * 6 +
                                     [i, i, i, vp, vp, vp, vp], None)
@@ -180,6 +182,10 @@ class HostModel:
 
     def fill_kv(self, ctx, seed, std=1.0):
         check(lib().mh_fill_kv(self.h, ctx, seed, std))
+
+    def kv_device(self, dtype=mc.BF16, page_size=16):
+        """Caches and attention on the GPU (dtype mc.F32, mc.F16 or mc.BF16)."""
+        check(lib().mh_kv_device(self.h, dtype, page_size))
 
     def timing(self):
         L = self.cfg["n_layers"]

@@ -152,3 +152,26 @@ def test_page_division_by_multiplication():
             for n in (q * d - 1, q * d, q * d + d - 1):
                 if 0 <= n < 2**31:
                     assert (n * m) >> (31 + l) == n // d
+
+
+def test_host_driver_without_a_gpu_keeps_its_cpu_caches():
+    """mh_kv_device refuses bad arguments, and where there is no GPU fails
+    loudly; the model's CPU attention then works as before."""
+    mh = pytest.importorskip("moe_host")
+    torch = pytest.importorskip("torch")
+    from helpers import TINY, tiny_model
+    g, attn, _ = tiny_model(2, seed=1)
+    m = mh.HostModel(TINY, batch=1, max_ctx=8)
+    m.set_globals(g["tok_emb"], g["final_norm_w"], g["lm_head"])
+    for l, a in enumerate(attn):
+        m.set_layer(l, a)
+    for args in ((9, 16), (mc.F32, 0)):
+        with pytest.raises(mc.MoeError) as e:
+            m.kv_device(*args)
+        assert e.value.code == INVALID
+    if not torch.cuda.is_available():
+        with pytest.raises(mc.MoeError):
+            m.kv_device(mc.F32, 16)
+    x = np.ones((2, TINY["d_model"]), np.float32)
+    assert np.isfinite(m.attention(0, x, 2)[0]).all()
+    m.close()

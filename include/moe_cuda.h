@@ -339,7 +339,9 @@ int moe_ffn_ep(int layer, const float* x_norm2, int T_local, float* x_inout,
  * `stream` and may be captured into a CUDA graph; none needs moe_cuda_init.
  * A call runs on the device that holds its first operand, whichever device is
  * current (the stream must be that device's). The calls keep nothing between
- * them: what they need beyond their operands is the caller's workspace.
+ * them: what they need beyond their operands is the caller's workspace. With
+ * CUDA's lazy module loading a kernel's first call on a device loads it: make
+ * one such call before a stream capture.
  *
  * A cache of n_pages pages of page_size tokens of n_kv heads. Element strides;
  * the head_dim elements of one head are contiguous. k and v 16-byte aligned,
@@ -416,6 +418,7 @@ int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k, long long 
  *     whatever they hold.
  * max_kv is what the longest row is expected to hold; it only sets how far a
  * row is split over the GPU (a longer row is right, but slower).
+ * At most 32768 query heads.
  * workspace: moe_paged_attention_workspace() bytes (0: none needed), 16-byte
  * aligned, no initial contents, one per call in flight: calls on two streams,
  * or two graphs that may run at the same time, need one each. */

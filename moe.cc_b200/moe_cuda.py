@@ -442,6 +442,8 @@ def _dev(t, dtype, n, what, device):
 
 def _rows(t, what, rows, heads, hd, device):
     """(pointer, row stride) of [rows][heads][head_dim] whose rows may lie apart."""
+    if t is None:
+        raise MoeError(MOE_ERR_INVALID, f"{what}: a tensor is wanted")
     st = t.stride()
     if t.shape != (rows, heads, hd) or t.get_device() != device or (
             (st[2] != 1 and hd > 1 or st[1] != hd and heads > 1) and rows):

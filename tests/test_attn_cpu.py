@@ -91,7 +91,7 @@ def test_rope_refuses(over, want):
 
 
 @pytest.mark.parametrize("over,want", [
-    (dict(rows=-1), INVALID), (dict(n_q=3), INVALID), (dict(n_q=0), INVALID), (dict(n_seq=-1), INVALID),
+    (dict(rows=-1), INVALID), (dict(n_q=3), INVALID), (dict(n_q=0), INVALID), (dict(n_q=32770), UNSUPPORTED), (dict(n_seq=-1), INVALID),
     (dict(max_pages=0), INVALID), (dict(rows=5), INVALID), (dict(max_kv=0), INVALID), (dict(q=None), INVALID),
     (dict(out=None), INVALID), (dict(pos=None), INVALID), (dict(table=None), INVALID), (dict(ldq=128), INVALID),
     (dict(ldo=260), INVALID), (dict(q=P + 2), INVALID), (dict(ws=None), INVALID), (dict(ws=P + 8), INVALID),

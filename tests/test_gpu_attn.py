@@ -288,6 +288,76 @@ def test_attention_in_place_repeatable_and_on_another_stream(gpu):
     assert torch.equal(q2, ref)
 
 
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("hint", [64, 2048, 6000])
+def test_attention_of_many_rows(gpu, dt, hint):
+    """More rows than are dealt evenly, of a few sequences of very different
+    lengths, with padding among them; the hint picks one CTA a row, or runs."""
+    lens = [5000, 1, 130, 2300]
+    q, k, v, table = make_attn(dt, 700, 4, 2, 64, 16, lens, seed=12)
+    rng = np.random.default_rng(2)
+    seq = rng.integers(-1, 4, 700)
+    pos = [int(rng.integers(-1, lens[s])) if s >= 0 else 3 for s in seq]
+    pos[5], seq[5] = 4999, 0
+    check_attn(q, k, v, table, pos, row_seq=seq.tolist(), max_kv=hint)
+
+
+def test_calls_that_follow_one_another_on_one_workspace(gpu):
+    """Calls of different sizes and types, each of which leaves its partial
+    results in the same workspace, with nothing waiting between them."""
+    sets = []
+    for i, (dt, rows, n_q, n_kv, hd, lens) in enumerate([
+            (torch.bfloat16, 3, 8, 2, 128, [4000, 100, 2500]), (torch.float16, 1, 16, 1, 64, [9000]),
+            (torch.float32, 2, 4, 4, 128, [3000, 70]), (torch.bfloat16, 2, 32, 1, 256, [2100, 2200])]):
+        q, k, v, table = make_attn(dt, rows, n_q, n_kv, hd, 16, lens, seed=20 + i)
+        pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32, device="cuda")
+        sets.append((q, k, v, table, pos, max(lens)))
+    alone = []
+    for q, k, v, table, pos, most in sets:
+        alone.append(run_attn(q, k, v, table, pos, 0.1, most)[0])
+        torch.cuda.synchronize()
+    need = max(mc.paged_attention_workspace(s[0].shape[0], s[0].shape[1], s[1], s[2], s[5]) for s in sets)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    outs = []
+    for _ in range(5):
+        for q, k, v, table, pos, most in sets:
+            out = torch.empty_like(q)
+            mc.paged_attention(q, k, v, table, pos, out, ws, most, 0.1)
+            outs.append(out)
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert torch.equal(out, alone[i % len(sets)])
+
+
+def test_a_step_written_just_before_it_is_read(gpu):
+    """Planning, append and attention follow one another on one stream over and
+    over with nothing in between: each sees what the one before it wrote."""
+    n_seq, nkv, hd, ps, n_pages = 7, 2, 64, 4, 400
+    i32 = dict(dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    steps = 60
+    kv = torch.randn(steps, 2, n_seq, nkv, hd, generator=g, device="cuda").bfloat16()
+    q = torch.randn(n_seq, 4, hd, generator=g, device="cuda").bfloat16()
+    past, new, head = torch.zeros(n_seq, **i32), torch.ones(n_seq, **i32), torch.zeros(1, **i32)
+    free, table, rows = torch.randperm(n_pages, generator=g, device="cuda").int(), torch.full((n_seq, 16), -1, **i32), torch.zeros(3, n_seq, **i32)
+    kc, vc = (torch.zeros(n_pages, ps, nkv, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    outs = torch.zeros(steps, n_seq, 4, hd, dtype=torch.bfloat16, device="cuda")
+    for t in range(steps):
+        mc.kv_plan(past, new, ps, n_pages, free, table, rows[0], rows[1], rows[2], kv_len=past, free_head=head, free_head_out=head)
+        mc.qk_norm_rope(None, kv[t, 0], kv[t, 1], kc, vc, rows[1], rows[2], None)
+        mc.paged_attention(q, kc, vc, table, rows[1], outs[t], None, 64, 0.125, row_seq=rows[0])
+    torch.cuda.synchronize()
+    K = kv[:, 0].double().repeat_interleave(2, 2)                       # [steps, seq, 4, hd]
+    V = kv[:, 1].double().repeat_interleave(2, 2)
+    for t in range(steps):
+        x = torch.einsum("shd,nshd->shn", q.double(), K[:t + 1]) * 0.125
+        w = torch.softmax(x, 2)
+        want = torch.einsum("shn,nshd->shd", w, V[:t + 1])
+        # |x| < 2^4: fp32 scores within 2^-14, weights with their 2^-16
+        assert near(outs[t], want, 2.0**-13 * torch.einsum("shn,nshd->shd", w, V[:t + 1].abs()))
+
+
 # ---- norm, rotation and append ---------------------------------------------------
 
 def rope_table(n, rot, theta=1e6):

@@ -47,6 +47,7 @@ namespace {
 constexpr int kMaxParts = 128;      // runs a row is split into at most
 constexpr int kPiece = 64;          // positions of the shortest run
 constexpr int kDealtRows = 512;     // rows whose work is dealt evenly
+constexpr int kRun = 8;             // pieces of the shortest run of more rows
 constexpr int kShort = 32;          // pieces up to which a cluster takes a row
 constexpr int kCluster = 8;         // CTAs of such a cluster at most
 enum { kRuns = 0, kDealt = 1, kClustered = 2 };
@@ -150,28 +151,34 @@ template <> __device__ __forceinline__ void store1<float>(void* p, long long i, 
 template <> __device__ __forceinline__ void store1<__nv_bfloat16>(void* p, long long i, float v) { ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ void store1<__half>(void* p, long long i, float v) { ((__half*)p)[i] = __float2half_rn(v); }
 
-// Shapes of one instantiation. HD: head_dim rounded up to 64, 128 or 256 (the
+// Shapes of one instantiation. HD: head_dim rounded up to 64, 96, 128 or 256 (the
 // columns between are zeros in shared memory); NT: 8-head column tiles.
 template <typename T, int HD, int NT>
 struct Shape {
   static constexpr bool wide = sizeof(T) == 4;
-  // The rows lie so that the fragment loads meet no bank conflicts and every
-  // 32-byte sector of a row stays one aligned 32-byte block: with rows 16 bytes
-  // off (a pitch of an odd number of pieces) each of their sectors crossed the
-  // crossbar twice. 16-bit rows: piece c of row r at c ^ (r & 7) (ldmatrix).
-  // fp32 rows: 8 words past a multiple of 32 (16-byte loads of 2 rows two
-  // apart, or of 4 rows 8 words each).
-  static constexpr int pitch = wide ? HD * 4 + 32 : HD * 2;
+  // Piece c (16 bytes) of row r lies at c ^ turn(r) of the row, so that the
+  // fragment loads meet no bank conflicts: 16-bit rows are read 8 at a time at
+  // one piece (ldmatrix), fp32 rows 4 pieces of 2 rows (K: rows two apart, see
+  // swap01) or 2 pieces of 4 rows (V) at a time. Rows pitched by an odd number
+  // of pieces would do too, but then every other row's 32-byte sectors are
+  // not aligned blocks and cross the crossbar twice.
+  static constexpr int pitch = HD * (int)sizeof(T);
+  static __device__ __forceinline__ constexpr int turn(int r) {
+    return wide ? 2 * (r & 3) : HD == 96 ? (r >> 1) & 3 : r & 7;   // 96: rows alternate between the banks' halves
+  }
   static constexpr int unit = kStep * pitch;       // the K or the V rows of a step
-  // Warps, ring units a warp and CTAs an SM: 8 to 12 warps, 100 to 150 KB of
-  // ring. 16-bit rows of 128, 32 rows of up to 8192 positions / one row of
-  // 131072: 3 CTAs of 4 warps 59.4 / 49.1 us, 2 of 4 60.8 / 49.0, 4 of 4 60.2 /
-  // 48.7, 1 of 8 64.5 / 50.0, 5 units in 2 CTAs of 4 60.7 / 49.5.
-  static constexpr int warps = wide && HD == 64 || !wide && HD == 256 ? 8 : 4;
-  static constexpr int units = HD == 64 || NT == 2 ? 5 : 3;
-  static constexpr int ctas = HD == 256 || wide && HD == 64 ? 1 : wide || NT == 2 ? 2 : 3;
+  // Warps, ring units a warp and CTAs an SM: 8 to 16 warps. 16-bit rows of
+  // 128, 32 rows of up to 8192 positions / one row of 131072: 3 CTAs of 4 warps
+  // 59.4 / 49.1 us, 2 of 4 60.8 / 49.0, 4 of 4 60.2 / 48.7, 1 of 8 64.5 / 50.0, 5
+  // units in 2 CTAs of 4 60.7 / 49.5. fp32, 32 rows of 2048 positions (268 MB):
+  // rows of 64 in 1 CTA of 8 warps with 5 units 97 us, 4 of 4 with 3 54; of 128
+  // in 2 of 4 with 3 73, 3 of 4 with 2 66; of 256 in 1 of 4 with 3 119, of 6 with
+  // 2 104.
+  static constexpr int warps = HD == 256 ? wide ? 6 : 8 : 4;
+  static constexpr int units = wide ? HD == 64 ? 3 : 2 : HD == 64 || NT == 2 ? 5 : 3;
+  static constexpr int ctas = HD == 256 ? 1 : wide ? HD == 64 ? 4 : 3 : NT == 2 ? 2 : HD == 96 ? 4 : 3;
   static constexpr int heads = 8 * NT;
-  static constexpr int q_pitch = HD * 4 + 64;      // fp32: Q's high and low parts, rows 16 words past
+  static constexpr int q_pitch = HD * 4 + 64;      // fp32: Q's high and low parts (4 pieces of 2 rows a load)
   static constexpr int q_bytes = wide ? 2 * heads * q_pitch : 0;
   static constexpr int ring = warps * units * unit;
   static constexpr int join = warps * heads * (HD + 2) * 4;
@@ -240,7 +247,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
 
   unsigned char* ring = sm + warp * (S::units * S::unit);
   const int* table = a.table + (long long)seq * a.max_pages;
-  constexpr int kPieces = HD * (int)sizeof(T) / 16;            // 16-byte pieces of a row
+  constexpr int kRow = HD * (int)sizeof(T) / 16;               // 16-byte pieces of a row
+  constexpr int kPieces = kRow == 12 ? 16 : kRow == 24 ? 32 : kRow;   // and the lanes that copy one
   const int pieces = a.hd * (int)sizeof(T) / 16;
   const char* kbase = (const char*)((const T*)a.k + kvh * a.head_stride);
   const char* vbase = (const char*)((const T*)a.v + kvh * a.head_stride);
@@ -248,11 +256,11 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
   const bool whole = a.page_size % kStep == 0;                 // a step never leaves its page
 
   // columns from head_dim to HD are zeros throughout: no copy touches them
-  if (pieces < kPieces) {
-    const int pad = kPieces - pieces;
+  if (pieces < kRow) {
+    const int pad = kRow - pieces;
     for (int i = lane; i < S::units * kStep * pad; i += 32) {
       const int r = i / pad, c = pieces + i % pad;
-      *reinterpret_cast<uint4*>(ring + r * S::pitch + 16 * (S::wide ? c : c ^ (r & 7))) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(ring + r * S::pitch + 16 * (c ^ S::turn(r))) = make_uint4(0, 0, 0, 0);
     }
   }
 
@@ -268,10 +276,10 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
   constexpr int kRows = kPieces <= 32 ? 32 / kPieces : 1;      // rows one instruction of the warp covers
   constexpr int kInsn = kStep * kPieces / 32;
   const int r0 = kPieces <= 32 ? lane / kPieces : 0, c0 = kPieces <= 32 ? lane % kPieces : lane;
-  const int d0 = r0 * S::pitch + 16 * (S::wide ? c0 : c0 ^ r0);
-  // where this lane's piece of row r0 + r goes (16-bit: kRows divides 8 and
-  // r0 < kRows, so (r0 + r) & 7 is r0 ^ (r & 7))
-  auto place = [&](int r, int c) { return S::wide ? d0 + r * S::pitch + 16 * c : (d0 ^ (16 * (r & 7))) + r * S::pitch; };
+  const int d0 = r0 * S::pitch + 16 * (c0 ^ S::turn(r0));
+  // where this lane's piece of row r0 + r goes (kRows is a power of two and
+  // r0 < kRows, so turn(r0 + r) is turn(r0) ^ turn(r))
+  auto place = [&](int r, int c) { return (d0 ^ (16 * S::turn(r))) + r * S::pitch + 16 * c; };
   auto issue = [&](const char* base, int i, int pg, int slot) -> unsigned {
     if (i >= mine) return 0u;
     const int t = t0 + (i * S::warps + warp) * kStep;
@@ -314,10 +322,11 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
 
   // The ring holds units K0 V0 K1 V1 ..., kAhead of them in flight; unit u lies
   // in slot u % units, and the copy of unit u + kAhead goes into the slot that
-  // unit u - 1 has just left.
+  // unit u - 1 has just left. For an even kAhead, K and V of step i are followed
+  // by K and V of step i + kSteps; for an odd one K by V and V by the next K.
   constexpr int kAhead = S::units - 1, kSteps = kAhead / 2;
-  static_assert(kAhead % 2 == 0, "K and V of a step are issued alike");
-  unsigned masks[kSteps + 1];
+  constexpr bool kOdd = kAhead & 1;
+  unsigned masks[kSteps + 1];                                  // of steps i, i + 1, ...
   int pg = page_at(0);
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
@@ -327,6 +336,10 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
     issue(vbase, i, pg, 2 * i + 1);
     copies_done();
     pg = next;
+  }
+  if constexpr (kOdd) {
+    masks[kSteps] = issue(kbase, kSteps, pg, 2 * kSteps);
+    copies_done();
   }
 
   // queries: 16-bit as B fragments in registers, fp32 as high and low parts in
@@ -380,8 +393,12 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
     wait_copies<kAhead - 1>();
     __syncwarp();
     const int next = page_at(i + kSteps + 1);
-    masks[kSteps] = issue(kbase, i + kSteps, pg, before(slot));
+    if constexpr (kOdd) issue(vbase, i + kSteps, pg, before(slot));
+    else masks[kSteps] = issue(kbase, i + kSteps, pg, before(slot));
     copies_done();
+    const unsigned mask = masks[0];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) masks[j] = masks[j + 1];
     const unsigned char* kst = ring + slot * S::unit;
     slot = after(slot);
 
@@ -394,8 +411,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
       for (int kk = 0; kk < HD / 16; ++kk) {
         // 16 columns: lane q4 holds columns 4 q4 .. 4 q4 + 3, the first two
         // as one k-step of 8, the other two as the next
-        const float4 x = *reinterpret_cast<const float4*>(kst + swap01(g) * S::pitch + 64 * kk + 16 * q4);
-        const float4 y = *reinterpret_cast<const float4*>(kst + (swap01(g) + 8) * S::pitch + 64 * kk + 16 * q4);
+        const unsigned char* at = kst + swap01(g) * S::pitch + ((64 * kk + 16 * q4) ^ (16 * S::turn(swap01(g))));
+        const float4 x = *reinterpret_cast<const float4*>(at);
+        const float4 y = *reinterpret_cast<const float4*>(at + 8 * S::pitch);
         const uint4 bh = *reinterpret_cast<const uint4*>(q_sm + g * S::q_pitch + 64 * kk + 16 * q4);
         const uint4 bl = *reinterpret_cast<const uint4*>(q_sm + (S::heads + g) * S::q_pitch + 64 * kk + 16 * q4);
         unsigned ah[4], al[4], ch[4], cl[4];
@@ -416,7 +434,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
     } else {
       // two accumulators a tile: half the chain of dependent products
       const unsigned ka = smem_u32(kst) + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::pitch;
-      const unsigned kx = 16 * ((lane >> 4) ^ (lane & 7));
+      const unsigned kx = 16 * ((lane >> 4) ^ S::turn(lane));
       float e[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -438,9 +456,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][j] += e[n][j];
     }
-    if (masks[0] != 0xffffu) {
+    if (mask != 0xffffu) {
       const int gt = S::wide ? swap01(g) : g;
-      const bool v0 = (masks[0] >> gt) & 1, v1 = (masks[0] >> (gt + 8)) & 1;
+      const bool v0 = (mask >> gt) & 1, v1 = (mask >> (gt + 8)) & 1;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -482,7 +500,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
 
     wait_copies<kAhead - 1>();
     __syncwarp();
-    issue(vbase, i + kSteps, pg, before(slot));
+    if constexpr (kOdd) masks[kSteps] = issue(kbase, i + kSteps + 1, next, before(slot));
+    else issue(vbase, i + kSteps, pg, before(slot));
     copies_done();
     pg = next;
     const unsigned char* vst = ring + slot * S::unit;
@@ -505,7 +524,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
         float4 x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          x[j] = *reinterpret_cast<const float4*>(vst + (q4 + 4 * j) * S::pitch + 128 * b + 16 * g);
+          x[j] = *reinterpret_cast<const float4*>(vst + (q4 + 4 * j) * S::pitch + ((128 * b + 16 * g) ^ (16 * S::turn(q4))));
         float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
         unsigned ah[2][4], al[2][4], ch[2][4], cl[2][4];
 #pragma unroll
@@ -542,7 +561,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
           pl[n][j] = turn8x8(lo);
         }
       const unsigned va = smem_u32(vst) + ((lane & 7) + (lane >> 4) * 8) * S::pitch;
-      const unsigned vx = 16 * (((lane >> 3) & 1) ^ (lane & 7));
+      const unsigned vx = 16 * (((lane >> 3) & 1) ^ S::turn(lane));
 #pragma unroll
       for (int mt = 0; mt < HD / 16; ++mt) {
         unsigned af[4];
@@ -554,8 +573,6 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
         }
       }
     }
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) masks[j] = masks[j + 1];
   }
 
   // ---- join the warps ----
@@ -652,17 +669,20 @@ __device__ __forceinline__ void clear_heads(const AttnArgs& a, int row, int head
 }
 
 // How the work is split, a "item" being a row's key-value head and tile:
-//   kDealt      The pieces of all items, one after another, are cut into as
-//               many equal stretches as there are CTAs, which is what the GPU
-//               holds at a time. A stretch may end one item and begin the next,
-//               so a ragged batch leaves no CTA waiting for the longest row.
-//               Every warp works the cut out for itself from the rows' lengths.
-//               A second launch joins the items' runs.
+//   kDealt      The CTAs are taken in groups, one for each key-value head (and
+//               tile), and the pieces of all rows, one row after another, are
+//               cut into as many equal stretches as there are groups, which is
+//               what the GPU holds at a time. A stretch may end one row and
+//               begin the next, so a ragged batch leaves no CTA waiting for the
+//               longest row; and the heads of a position, neighbours in memory,
+//               are read at about the same time. Every warp works the cut out
+//               for itself from the rows' lengths. A second launch joins the
+//               items' runs.
 //   kClustered  An item is a cluster's: each CTA takes an equal run, and they
 //               join through distributed shared memory. One launch, for short
 //               contexts, where the second one would be most of the time.
-//   kRuns       A CTA takes one run of 8 pieces at least (or, with room for one
-//               part only, the item): for rows too many to be dealt.
+//   kRuns       A CTA takes one run of kRun pieces at least (or, with room for
+//               one part only, the item): for rows too many to be dealt.
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(Shape<T, HD, NT>::warps * 32, Shape<T, HD, NT>::ctas)
 paged_attn_kernel(const AttnArgs a) {
@@ -673,13 +693,13 @@ paged_attn_kernel(const AttnArgs a) {
   const int lane = threadIdx.x & 31, kt = a.n_kv * a.tiles;
 
   int row, len, u;                  // the current row, its positions and pieces
-  int run_part = 0;
-  int base, w, w1, stretch;         // where its items' pieces begin; this CTA's pieces; pieces a CTA
   if (a.mode == kDealt) {
     for (row = blockIdx.x; row < a.rows; row += gridDim.x)
       if (length_of(a, row) == 0) clear_heads<T>(a, row, 0, a.n_q);
+    const int group = blockIdx.x / kt, groups = gridDim.x / kt, i = blockIdx.x - group * kt;
     const int per = (a.rows + 31) / 32, r0 = min(lane * per, a.rows), r1 = min(r0 + per, a.rows);
     int sum = 0, most = 0, last_len = 0;
+#pragma unroll 4
     for (int r = r0; r < r1; ++r) {
       last_len = length_of(a, r);
       const int n = pieces_of(last_len);
@@ -692,57 +712,57 @@ paged_attn_kernel(const AttnArgs a) {
       const int x = __shfl_up_sync(~0u, upto, o);
       if (lane >= o) upto += x;
     }
-    const int total = __shfl_sync(~0u, upto, 31) * kt;
+    const int total = __shfl_sync(~0u, upto, 31);
     most = __reduce_max_sync(~0u, most);
-    // long enough that no item is cut into more than a.parts runs: u pieces
+    // long enough that no row is cut into more than a.parts runs: u pieces
     // meet at most (u - 2) / stretch + 2 stretches
-    stretch = max(max(1, (total - 1) / (int)gridDim.x + 1), (most + a.parts - 3) / (a.parts - 1));
-    if ((long long)blockIdx.x * stretch >= total) return;
-    w = blockIdx.x * stretch;
-    w1 = total - w < stretch ? total : w + stretch;
-    const int owner = __ffs(__ballot_sync(~0u, upto * kt > w)) - 1;
+    const int stretch = max(max(1, (total - 1) / groups + 1), (most + a.parts - 3) / (a.parts - 1));
+    if ((long long)group * stretch >= total) return;
+    int w = group * stretch;                       // this group's pieces
+    const int w1 = total - w < stretch ? total : w + stretch;
+    const int owner = __ffs(__ballot_sync(~0u, upto > w)) - 1;
     row = owner * per;
-    base = __shfl_sync(~0u, upto - sum, owner) * kt;
+    int base = __shfl_sync(~0u, upto - sum, owner);   // where the row's pieces begin
     len = per == 1 ? __shfl_sync(~0u, last_len, owner) : length_of(a, row);
     u = pieces_of(len);
-  } else {
-    run_part = blockIdx.x % a.parts;
-    const int item = blockIdx.x / a.parts, i = item % kt;
-    row = item / kt;
-    len = length_of(a, row);
-    if (len < 0) return;
-    if (len == 0) {
-      const int tile = i % a.tiles;
-      if (run_part == 0)
-        clear_heads<T>(a, row, i / a.tiles * a.group + tile * S::heads, min(S::heads, a.group - tile * S::heads));
-      return;
+    for (;;) {
+      while (base + u <= w) {
+        base += u;
+        if (++row >= a.rows) return;
+        len = length_of(a, row);
+        u = pieces_of(len);
+      }
+      const int off = w - base, n = min(u - off, w1 - w);
+      const int first = base / stretch, last = (base + u - 1) / stretch, part = group - first;
+      // Lengths that somebody changes while the kernel runs make the warps' cuts
+      // disagree; the result is then anything, but nothing outside is touched.
+      if (off < 0 || part < 0 || part >= a.parts) return;
+      attend<T, HD, NT>(a, sm, row, i / a.tiles, i % a.tiles, off * kPiece, min(len, (off + n) * kPiece), part,
+                        last - first + 1);
+      w += n;
+      if (w >= w1) return;
+      __syncthreads();              // the ring is free again
     }
-    u = pieces_of(len);
-    stretch = (u - 1) / a.parts + 1;
-    if (a.mode == kRuns && a.parts > 1) stretch = max(8, stretch);
-    w = min(run_part * stretch, u);
-    w1 = min(w + stretch, u);
-    // a cluster's CTA without a run of its own still takes part in the join
-    if (w >= w1 && a.mode != kClustered) return;
-    const int parts = a.mode == kClustered ? a.parts : (u - 1) / stretch + 1;
-    attend<T, HD, NT>(a, sm, row, i / a.tiles, i % a.tiles, min(len, w * kPiece), min(len, w1 * kPiece), run_part, parts);
-    if (a.mode == kClustered && parts > 1) cluster_sync();     // the others may still be reading here
+  }
+  const int run_part = blockIdx.x % a.parts, item = blockIdx.x / a.parts, i = item % kt;
+  row = item / kt;
+  len = length_of(a, row);
+  if (len <= 0) {
+    const int tile = i % a.tiles;
+    if (len == 0 && run_part == 0)
+      clear_heads<T>(a, row, i / a.tiles * a.group + tile * S::heads, min(S::heads, a.group - tile * S::heads));
+    if (a.mode == kClustered) { cluster_sync(); cluster_sync(); }
     return;
   }
-  for (;;) {
-    while (base + u * kt <= w) {
-      base += u * kt;
-      len = length_of(a, ++row);
-      u = pieces_of(len);
-    }
-    const int item = (w - base) / u, off = (w - base) - item * u, n = min(u - off, w1 - w), start = base + item * u;
-    const int first = start / stretch, last = (start + u - 1) / stretch;
-    attend<T, HD, NT>(a, sm, row, item / a.tiles, item % a.tiles, off * kPiece, min(len, (off + n) * kPiece),
-                      blockIdx.x - first, last - first + 1);
-    w += n;
-    if (w >= w1) return;
-    __syncthreads();                // the ring is free again
-  }
+  u = pieces_of(len);
+  int run = (u - 1) / a.parts + 1;
+  if (a.mode == kRuns && a.parts > 1) run = max(kRun, run);
+  const int w = min(run_part * run, u), w1 = min(w + run, u);
+  // a cluster's CTA without a run of its own still takes part in the join
+  if (w >= w1 && a.mode != kClustered) return;
+  attend<T, HD, NT>(a, sm, row, i / a.tiles, i % a.tiles, min(len, w * kPiece), min(len, w1 * kPiece), run_part,
+                    a.mode == kClustered ? a.parts : (u - 1) / run + 1);
+  if (a.mode == kClustered) cluster_sync();        // the others may still be reading here
 }
 
 // Joins the runs of a row: a block per (row, query head), the runs dealt to
@@ -844,17 +864,23 @@ int head_tile(int dtype, int hd, int group) {
 }
 
 // The split of a call, from what the host knows of it, and the parts that a
-// row's head may have. Short contexts: clusters that together are about four
-// CTAs per SM, of one CTA where the items alone are that many.
+// row's head may have. Short contexts: clusters of as many CTAs as bring their
+// number to 200, one where the items alone are that many (clusters are slow to
+// place: 16 rows of 1024 positions take 10.3 us in 256 CTAs, 15.0 in 512; 64
+// rows 25 us in 256, 34 in 1024).
 struct Split { int mode, parts; };
 Split split_of(long long items, int rows, int max_kv) {
   const int pieces = (max_kv - 1) / kPiece + 1;
   if (pieces <= kShort) {
     int n = 1;
-    while (n < kCluster && n < pieces && items * n < 592) n *= 2;
+    while (n < kCluster && n < pieces && items * n < 200) n *= 2;
     return {n > 1 ? kClustered : kRuns, n};
   }
-  return {rows <= kDealtRows ? kDealt : kRuns, pieces < kMaxParts ? pieces : kMaxParts};
+  if (rows > kDealtRows) {
+    const int runs = (pieces - 1) / kRun + 1;
+    return {kRuns, runs < kMaxParts ? runs : kMaxParts};
+  }
+  return {kDealt, pieces < kMaxParts ? pieces : kMaxParts};
 }
 
 int sm_count(int device) {
@@ -882,12 +908,12 @@ cudaError_t launch_attn(AttnArgs a, int max_kv, int device, cudaStream_t st) {
   const long long items = (long long)a.rows * a.n_kv * a.tiles, sms = sm_count(device);
   long long grid = items * a.parts;
   if (a.mode == kDealt) {
-    // what the GPU holds at a time; where an item's parts are too few for
-    // that, the largest whole number of CTAs per SM that they allow; and no
-    // more CTAs than pieces
-    const long long room = sms * S::ctas, most = items * (a.parts - 1), all = items * ((max_kv - 1) / kPiece + 1);
-    grid = most >= room ? room : most >= sms ? most / sms * sms : most;
-    if (grid > all) grid = all;
+    // as many groups as the GPU holds at a time, if the rows have parts and
+    // pieces for them
+    const long long kt = (long long)a.n_kv * a.tiles, fit = sms * S::ctas / kt, pieces = (max_kv - 1) / kPiece + 1;
+    long long groups = fit < a.rows * (a.parts - 1ll) ? fit : a.rows * (a.parts - 1ll);
+    if (groups > a.rows * pieces) groups = a.rows * pieces;
+    grid = (groups > 1 ? groups : 1) * kt;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(S::warps * 32); cfg.dynamicSmemBytes = S::smem; cfg.stream = st;
@@ -912,9 +938,12 @@ cudaError_t launch_attn(AttnArgs a, int max_kv, int device, cudaStream_t st) {
 template <typename T>
 cudaError_t launch_type(const AttnArgs& a, int tile, int max_kv, int device, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    if (tile == 16) return a.hd <= 64 ? launch_attn<T, 64, 2>(a, max_kv, device, st) : launch_attn<T, 128, 2>(a, max_kv, device, st);
+    if (tile == 16 && a.hd <= 64) return launch_attn<T, 64, 2>(a, max_kv, device, st);
+    if (tile == 16 && a.hd <= 96) return launch_attn<T, 96, 2>(a, max_kv, device, st);
+    if (tile == 16) return launch_attn<T, 128, 2>(a, max_kv, device, st);
   }
   if (a.hd <= 64) return launch_attn<T, 64, 1>(a, max_kv, device, st);
+  if (a.hd <= 96) return launch_attn<T, 96, 1>(a, max_kv, device, st);
   if (a.hd <= 128) return launch_attn<T, 128, 1>(a, max_kv, device, st);
   return launch_attn<T, 256, 1>(a, max_kv, device, st);
 }
@@ -964,7 +993,7 @@ extern "C" int moe_paged_attention_dev(const void* q, long long ldq, const MoeKv
   a.mode = sp.mode;
   // pieces are numbered in 32 bits where they are dealt out
   const long long pieces = (long long)max_pages * cache->page_size / kPiece + 1;
-  if (a.mode == kDealt && items * pieces > INT32_MAX) a.mode = kRuns;
+  if (a.mode == kDealt && rows * pieces > INT32_MAX) a.mode = kRuns;
   if (items * a.parts > INT32_MAX || (long long)rows * n_q > INT32_MAX)
     return at::fail(MOE_ERR_UNSUPPORTED, "%s: too many rows and heads for one launch", who);
   const size_t need = moe_paged_attention_workspace(rows, n_q, cache, max_kv);

@@ -8,6 +8,7 @@ import pytest
 
 import moe_cuda as mc
 
+DEALT = 512                   # rows whose work is dealt evenly
 P = 0x7000_0000_0000          # a 16-byte aligned address that nothing reads
 INVALID, UNSUPPORTED = mc.MOE_ERR_INVALID, mc.MOE_ERR_UNSUPPORTED
 
@@ -102,14 +103,15 @@ def test_attention_refuses(over, want):
 
 def test_attention_workspace_size():
     """None for contexts up to 2048 positions (one launch); above, a row of
-    head_dim + 2 floats per query head and 64 positions, at most 128."""
+    head_dim + 2 floats per query head and 64 positions (512 where rows are too
+    many to be dealt out), at most 128."""
     ws = mc.lib().moe_paged_attention_workspace
     for rows, n_q, max_kv in ((1, 2, 1), (4, 4, 64), (1, 32, 2048), (600, 4, 1000), (0, 4, 4096), (4, 3, 4096), (4, 4, 0)):
         assert ws(rows, n_q, C.byref(cache()), max_kv) == 0
     for rows, n_q, max_kv in ((1, 2, 2049), (1, 32, 1 << 20), (33, 8, 8192), (600, 4, 5000), (1, 2, 2**31 - 1)):
         n = ws(rows, n_q, C.byref(cache()), max_kv)
         one = rows * n_q * (64 + 2) * 4
-        assert n == min(128, -(-max_kv // 64)) * one + 16
+        assert n == min(128, -(-max_kv // (64 if rows <= DEALT else 512))) * one + 16
 
 
 @pytest.mark.parametrize("over,want", [

@@ -671,13 +671,13 @@ __device__ __forceinline__ void clear_heads(const AttnArgs& a, int row, int head
 // How the work is split, a "item" being a row's key-value head and tile:
 //   kDealt      The CTAs are taken in groups, one for each key-value head (and
 //               tile), and the pieces of all rows, one row after another, are
-//               cut into as many equal stretches as there are groups, which is
-//               what the GPU holds at a time. A stretch may end one row and
-//               begin the next, so a ragged batch leaves no CTA waiting for the
-//               longest row; and the heads of a position, neighbours in memory,
-//               are read at about the same time. Every warp works the cut out
-//               for itself from the rows' lengths. A second launch joins the
-//               items' runs.
+//               cut into as many stretches, equal to a piece, as there are
+//               groups, which is what the GPU holds at a time. A stretch may end
+//               one row and begin the next, so a ragged batch leaves no CTA
+//               waiting for the longest row; and the heads of a position,
+//               neighbours in memory, are read at about the same time. Every
+//               warp works the cut out for itself from the rows' lengths. A
+//               second launch joins the items' runs.
 //   kClustered  An item is a cluster's: each CTA takes an equal run, and they
 //               join through distributed shared memory. One launch, for short
 //               contexts, where the second one would be most of the time.
@@ -696,7 +696,8 @@ paged_attn_kernel(const AttnArgs a) {
   if (a.mode == kDealt) {
     for (row = blockIdx.x; row < a.rows; row += gridDim.x)
       if (length_of(a, row) == 0) clear_heads<T>(a, row, 0, a.n_q);
-    const int group = blockIdx.x / kt, groups = gridDim.x / kt, i = blockIdx.x - group * kt;
+    const unsigned group = blockIdx.x / kt;
+    const int i = blockIdx.x - group * kt;
     const int per = (a.rows + 31) / 32, r0 = min(lane * per, a.rows), r1 = min(r0 + per, a.rows);
     int sum = 0, most = 0, last_len = 0;
 #pragma unroll 4
@@ -712,14 +713,18 @@ paged_attn_kernel(const AttnArgs a) {
       const int x = __shfl_up_sync(~0u, upto, o);
       if (lane >= o) upto += x;
     }
-    const int total = __shfl_sync(~0u, upto, 31);
+    const unsigned total = __shfl_sync(~0u, upto, 31);
     most = __reduce_max_sync(~0u, most);
-    // long enough that no row is cut into more than a.parts runs: u pieces
-    // meet at most (u - 2) / stretch + 2 stretches
-    const int stretch = max(max(1, (total - 1) / groups + 1), (most + a.parts - 3) / (a.parts - 1));
-    if ((long long)group * stretch >= total) return;
-    int w = group * stretch;                       // this group's pieces
-    const int w1 = total - w < stretch ? total : w + stretch;
+    if (total == 0) return;
+    // Group g takes pieces floor(g total / G) to floor((g + 1) total / G), so
+    // piece x is group floor(((x + 1) G - 1) / total)'s. u pieces meet at most
+    // ceil((u - 1) G / total) + 1 groups: G is kept so low that this is at most
+    // a.parts. (The host sees to it that these products stay below 2^32.)
+    unsigned G = min((unsigned)(gridDim.x / kt), total);
+    if (most > 1) G = min(G, max(1u, (a.parts - 1) * total / (most - 1)));
+    if (group >= G) return;
+    int w = (int)(group * total / G);              // this group's pieces
+    const int w1 = (int)((group + 1) * total / G);
     const int owner = __ffs(__ballot_sync(~0u, upto > w)) - 1;
     row = owner * per;
     int base = __shfl_sync(~0u, upto - sum, owner);   // where the row's pieces begin
@@ -733,7 +738,8 @@ paged_attn_kernel(const AttnArgs a) {
         u = pieces_of(len);
       }
       const int off = w - base, n = min(u - off, w1 - w);
-      const int first = base / stretch, last = (base + u - 1) / stretch, part = group - first;
+      const int first = (int)(((base + 1u) * G - 1) / total), last = (int)(((unsigned)(base + u) * G - 1) / total);
+      const int part = (int)group - first;
       // Lengths that somebody changes while the kernel runs make the warps' cuts
       // disagree; the result is then anything, but nothing outside is touched.
       if (off < 0 || part < 0 || part >= a.parts) return;
@@ -913,6 +919,7 @@ cudaError_t launch_attn(AttnArgs a, int max_kv, int device, cudaStream_t st) {
     const long long kt = (long long)a.n_kv * a.tiles, fit = sms * S::ctas / kt, pieces = (max_kv - 1) / kPiece + 1;
     long long groups = fit < a.rows * (a.parts - 1ll) ? fit : a.rows * (a.parts - 1ll);
     if (groups > a.rows * pieces) groups = a.rows * pieces;
+    if (groups > 1023) groups = 1023;
     grid = (groups > 1 ? groups : 1) * kt;
   }
   cudaLaunchConfig_t cfg = {};
@@ -991,9 +998,10 @@ extern "C" int moe_paged_attention_dev(const void* q, long long ldq, const MoeKv
   const Split sp = split_of(items, rows, max_kv);
   a.parts = sp.parts;
   a.mode = sp.mode;
-  // pieces are numbered in 32 bits where they are dealt out
+  // where pieces are dealt out, their number times that of the groups (fewer
+  // than 1024) has 32 bits
   const long long pieces = (long long)max_pages * cache->page_size / kPiece + 1;
-  if (a.mode == kDealt && rows * pieces > INT32_MAX) a.mode = kRuns;
+  if (a.mode == kDealt && rows * pieces > INT32_MAX / 1024) a.mode = kRuns;
   if (items * a.parts > INT32_MAX || (long long)rows * n_q > INT32_MAX)
     return at::fail(MOE_ERR_UNSUPPORTED, "%s: too many rows and heads for one launch", who);
   const size_t need = moe_paged_attention_workspace(rows, n_q, cache, max_kv);

@@ -156,6 +156,33 @@ def test_page_division_by_multiplication():
                     assert (n * m) >> (31 + l) == n // d
 
 
+def test_pieces_are_dealt_whole_and_in_few_parts():
+    """The arithmetic by which the attention deals the rows' 64-position pieces
+    to groups of CTAs: every piece to one group, a row's groups in succession
+    and no more of them than it has room for, shares equal to a piece."""
+    rng = np.random.default_rng(1)
+    for _ in range(400):
+        rows = int(rng.integers(1, 40))
+        pieces = rng.integers(0, int(2 ** rng.uniform(0, 12)) + 1, rows)
+        parts, grid = int(rng.integers(33, 129)), int(rng.integers(1, 150))
+        total, most = int(pieces.sum()), int(pieces.max())
+        if total == 0:
+            continue
+        G = min(grid, total)
+        if most > 1:
+            G = min(G, max(1, (parts - 1) * total // (most - 1)))
+        cuts = [g * total // G for g in range(G + 1)]
+        assert cuts[0] == 0 and cuts[-1] == total and {b - a for a, b in zip(cuts, cuts[1:])} <= {total // G, -(-total // G)}
+        owner = np.searchsorted(np.array(cuts), np.arange(total), side="right") - 1
+        assert all(((x + 1) * G - 1) // total == owner[x] for x in range(total))
+        base = 0
+        for u in pieces.tolist():
+            if u:
+                first, last = ((base + 1) * G - 1) // total, ((base + u) * G - 1) // total
+                assert last - first + 1 <= parts
+            base += u
+
+
 def test_host_driver_without_a_gpu_keeps_its_cpu_caches():
     """mh_kv_device refuses bad arguments, and where there is no GPU fails
     loudly; the model's CPU attention then works as before."""

@@ -21,6 +21,8 @@
  *     exactly 0 to the sum and 0*v to the output, so stopping at the
  *     query's own position gives the same values.
  * glibc's expf/sqrtf/powf/cosf/sinf are called as the reference calls them.
+ * With mh_kv_device the norm and rotation of the heads, the caches and the
+ * attention run on the GPU instead; the projections stay here.
  */
 #define _POSIX_C_SOURCE 200809L
 #include <math.h>

@@ -407,10 +407,10 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
   float s;
   if (a.renorm) {
     // only ratios matter: from the largest chosen logit, so that they survive
-    // where the scores themselves would underflow (far below 0 the sigmoid is
-    // the exponential)
+    // where the scores themselves would underflow (the sigmoid is
+    // exp(x) / (1 + exp(x)))
     const float m = value_of(__reduce_max_sync(~0u, chosen >= 0 ? key_of(xe) : 0u));
-    s = a.softmax || m < -40.f ? soft(xe, m) : sigm(xe);
+    s = a.softmax ? soft(xe, m) : m > 0.f ? sigm(xe) : soft(xe, m) / (1.0f + expf(xe));
     if (chosen < 0) s = 0.f;
     const float sum = warp_sum_of(s);
     s = sum > 0.f ? s / sum : 0.f;

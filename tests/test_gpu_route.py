@@ -146,8 +146,11 @@ def test_many_tokens_choose_as_64_bits_do(gpu, score):
 def test_ratios_survive_where_scores_underflow(gpu):
     x = torch.full((2, 32), -300.0)
     x[0, 3], x[0, 4], x[1, 5] = -299.0, -299.5, 200.0
+    y = torch.full((2, 32), -91.0)
+    y[0, 3], y[1, 5], y[1, 6] = -10.0, 1.0, -70.0      # some of the chosen underflow, their share does not
     for score in ("sigmoid", "softmax"):
         check(x.cuda(), 4, None, score)
+        check(y.cuda(), 6, None, score)
     bias = torch.zeros(32)
     bias[8:12] = 5.0                                # the chosen are not the likely ones
     check(x.cuda(), 4, bias.cuda(), "softmax")

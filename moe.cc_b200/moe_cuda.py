@@ -8,11 +8,13 @@ tensors go through the device-pointer entries (pointers and a stream only —
 torch is plumbing for device memory, never part of the computation).
 
 There is no CPU fallback: if the library is missing or no GPU is present the
-calls fail loudly.
+calls fail loudly. The calls of a decode step around the MoE block (kv_plan,
+qk_norm_rope, paged_attention, route) go through a CPython extension instead
+of ctypes.
 """
 import ctypes as C
+import importlib.util
 import os
-import struct
 
 import numpy as np
 
@@ -25,7 +27,6 @@ Q8, Q4 = 2, 3
 HOST_PTRS, DEVICE_PTRS, FORCE_GEMV, FORCE_GEMM = 0x1, 0x0, 0x4, 0x8
 SEQ_RESIDUAL, GIVEN_TOPK = 0x10, 0x20
 F32, F16, BF16 = 0, 1, 4
-ROUTE_SCORES = {"softmax": 0, "sigmoid": 1}
 
 # Every symbol include/moe_cuda.h declares (checked by the CPU test suite).
 EXPORTS = (
@@ -405,180 +406,44 @@ def moe_ffn_ep(layer, x_norm2, x_inout, stream=None):
 
 
 # ---- attention over a paged key-value cache, expert routing ------------------
-# torch CUDA tensors; `stream` as in the calls above. A tensor of the wrong type,
-# place or layout is refused here, before its pointer is handed on.
+# kv_plan, qk_norm_rope, paged_attention and route take torch CUDA tensors and
+# `stream` as the calls above, and live in a CPython extension (py/moe_fast.c,
+# which also documents them): it refuses a tensor of the wrong type, place or
+# layout before its pointer is handed on. It is loaded with the first of them.
 
-class _Types:
-    """torch's types, looked up when the first tensor comes (this module does
-    not import torch)."""
-    elem = None
-
-    @classmethod
-    def load(cls):
-        import torch
-        cls.i32, cls.f32 = torch.int32, torch.float32
-        cls.elem = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_FAST = ("kv_plan", "qk_norm_rope", "paged_attention", "route")
+FAST_PATH = os.path.join(HERE, "_moe_fast.so")
 
 
-def _elem(t, what):
-    if _Types.elem is None:
-        _Types.load()
-    d = _Types.elem.get(t.dtype)
-    if d is None:
-        raise MoeError(MOE_ERR_INVALID, f"{what}: float32, float16 or bfloat16 is wanted, got {t.dtype}")
-    return d
-
-
-def _dev(t, dtype, n, what, device):
-    """Pointer of a contiguous tensor of n elements of the given type on CUDA
-    device number `device`; None passes through."""
-    if t is None:
-        return None
-    if t.dtype is not dtype or t.numel() != n or t.get_device() != device or not t.is_contiguous():
-        raise MoeError(MOE_ERR_INVALID, f"{what}: a contiguous {dtype} tensor of {n} elements on cuda:{device} is "
-                                        f"wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _rows(t, what, rows, heads, hd, device):
-    """(pointer, row stride) of [rows][heads][head_dim] whose rows may lie apart."""
-    if t is None:
-        raise MoeError(MOE_ERR_INVALID, f"{what}: a tensor is wanted")
-    st = t.stride()
-    if t.shape != (rows, heads, hd) or t.get_device() != device or (
-            (st[2] != 1 and hd > 1 or st[1] != hd and heads > 1) and rows):
-        raise MoeError(MOE_ERR_INVALID, f"{what}: [{rows}][{heads}][{hd}] on cuda:{device} with contiguous rows is wanted, "
-                                        f"got {tuple(t.shape)}, strides {st} on {t.device}")
-    return t.data_ptr(), (st[0] if rows > 1 else heads * hd)
-
-
-def _cuda_device(t, what):
-    """The number of the CUDA device that holds t."""
-    if not t.is_cuda:
-        raise MoeError(MOE_ERR_INVALID, f"{what}: a CUDA tensor is wanted")
-    if _Types.elem is None:
-        _Types.load()
-    return t.get_device()
-
-
-# MoeKvCache's bytes: packing them costs half of filling the ctypes structure
-_CACHE = struct.Struct("@PPiiiiiqqq")
-assert _CACHE.size == C.sizeof(MoeKvCache)
-
-
-def _cache(k, v):
-    """(MoeKvCache as bytes, device, dtype, n_kv, head_dim) of two cache tensors."""
-    shape, sk, sv = k.shape, k.stride(), v.stride()
-    if len(shape) == 4 and sk != sv and 1 in shape:          # the stride of a dimension of one says nothing
-        sk, sv = ([0 if n == 1 else s for n, s in zip(shape, st)] for st in (sk, sv))
-    device, dtype = k.get_device(), k.dtype
-    if len(shape) != 4 or shape != v.shape or dtype is not v.dtype or sk != sv or device != v.get_device():
-        raise MoeError(MOE_ERR_INVALID, "kv cache: k and v of one type and layout, [n_pages][page_size][n_kv][head_dim]")
-    n, ps, nkv, hd = shape
-    if sk[3] != 1 and hd > 1:
-        raise MoeError(MOE_ERR_INVALID, "kv cache: the head dimension must be contiguous")
-    c = _CACHE.pack(k.data_ptr(), v.data_ptr(), _elem(k, "kv cache"), n, ps, nkv, hd, sk[0], sk[1], sk[2])
-    return c, device, dtype, nkv, hd
+def __getattr__(name):
+    if name not in _FAST:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    lib()
+    if not os.path.exists(FAST_PATH):
+        raise MoeError(MOE_ERR_NOT_INIT, f"{FAST_PATH} is not built (run make -C moe.cc_b200 where Python's headers are)")
+    spec = importlib.util.spec_from_file_location("_moe_fast", FAST_PATH)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m._set_error(MoeError)
+    for n in _FAST:
+        globals()[n] = getattr(m, n)
+    return globals()[name]
 
 
 def kv_cache(k, v):
     """MoeKvCache of two tensors [n_pages][page_size][n_kv][head_dim] of one
     type and one layout, the last dimension contiguous, the others in any
     order. The tensors must outlive it."""
-    return MoeKvCache.from_buffer_copy(_cache(k, v)[0])
-
-
-def kv_plan(past_len, new_len, page_size, n_pages, free_pages, block_table, row_seq, row_pos, row_slot, kv_len=None,
-            free_head=None, free_head_out=None, status=None, stream=None):
-    """moe_kv_plan_dev: int32 tensors; past_len may be None (nothing held yet)."""
-    dev, i32 = _cuda_device(block_table, "kv_plan"), _Types.i32
-    (n, mp), cap, free = block_table.shape, row_seq.numel(), free_pages.numel()
-    check(lib().moe_kv_plan_dev(
-        _dev(past_len, i32, n, "past_len", dev), _dev(new_len, i32, n, "new_len", dev), n, page_size, n_pages,
-        _dev(free_pages, i32, free, "free_pages", dev), free, _dev(free_head, i32, 1, "free_head", dev),
-        _dev(block_table, i32, n * mp, "block_table", dev), mp, _dev(kv_len, i32, n, "kv_len", dev),
-        _dev(row_seq, i32, cap, "row_seq", dev), _dev(row_pos, i32, cap, "row_pos", dev),
-        _dev(row_slot, i32, cap, "row_slot", dev), cap, _dev(free_head_out, i32, 1, "free_head_out", dev),
-        _dev(status, i32, 3, "status", dev), _stream(stream)))
-
-
-def qk_norm_rope(q, k, v, k_cache, v_cache, row_pos, row_slot, q_out, rope=None, q_norm=None, k_norm=None, eps=1e-6,
-                 stream=None):
-    """moe_qk_norm_rope_dev. q [rows][n_q][head_dim] (None: keys and values
-    only), k, v [rows][n_kv][head_dim], rows of one stride each; rope
-    [positions][rot_dim] fp32, the cosines then the sines; row_slot None:
-    queries only (k, v are then not read and may be None)."""
-    c, dev, ct, n_kv, hd = _cache(k_cache, v_cache)
-    _cuda_device(k_cache, "qk_norm_rope")
-    i32, f32 = _Types.i32, _Types.f32
-    x = q if q is not None else k
-    rows, xt, dt = x.shape[0], x.dtype, _elem(x, "q")
-    qp = op = kp = vp = None
-    ldq = ldo = ldk = ldv = n_q = 0
-    if q is not None:
-        n_q = q.shape[1]
-        qp, ldq = _rows(q, "q", rows, n_q, hd, dev)
-        op, ldo = _rows(q_out, "q_out", rows, n_q, hd, dev)
-        if q_out.dtype is not ct:
-            raise MoeError(MOE_ERR_INVALID, "q_out: the cache's type is wanted")
-    if row_slot is not None:
-        kp, ldk = _rows(k, "k", rows, n_kv, hd, dev)
-        vp, ldv = _rows(v, "v", rows, n_kv, hd, dev)
-        if k.dtype is not xt or v.dtype is not xt:
-            raise MoeError(MOE_ERR_INVALID, "q, k and v: one type is wanted")
-    n_rope, rot = rope.shape if rope is not None else (0, 0)
-    check(lib().moe_qk_norm_rope_dev(
-        qp, ldq, kp, ldk, vp, ldv, dt, rows, n_q, _dev(q_norm, f32, hd, "q_norm", dev),
-        _dev(k_norm, f32, hd, "k_norm", dev), eps, _dev(rope, f32, n_rope * rot, "rope", dev), rot, n_rope,
-        _dev(row_pos, i32, rows, "row_pos", dev), _dev(row_slot, i32, rows, "row_slot", dev), op, ldo,
-        c, _stream(stream)))
+    dt = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}.get(str(k.dtype))
+    sk, sv = ([0 if n == 1 else s for n, s in zip(t.shape, t.stride())] for t in (k, v))   # of a dimension of one it says nothing
+    if dt is None or k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or sk != sv or sk[3] > 1:
+        raise MoeError(MOE_ERR_INVALID, "kv cache: k and v of one type and layout, [n_pages][page_size][n_kv][head_dim]")
+    return MoeKvCache(k.data_ptr(), v.data_ptr(), dt, *k.shape, *sk[:3])
 
 
 def paged_attention_workspace(rows, n_q, k_cache, v_cache, max_kv):
     """Bytes of workspace of a paged_attention call (0: none)."""
-    return lib().moe_paged_attention_workspace(rows, n_q, _cache(k_cache, v_cache)[0], max_kv)
-
-
-def paged_attention(q, k_cache, v_cache, block_table, row_pos, out, workspace, max_kv, scale, lse=None, row_seq=None,
-                    stream=None):
-    """moe_paged_attention_dev. q, out [rows][n_q][head_dim]; workspace: a
-    contiguous tensor of any type (None where none is needed)."""
-    c, dev, dt, _, hd = _cache(k_cache, v_cache)
-    _cuda_device(k_cache, "paged_attention")
-    i32 = _Types.i32
-    rows, n_q = q.shape[:2]
-    qp, ldq = _rows(q, "q", rows, n_q, hd, dev)
-    op, ldo = _rows(out, "out", rows, n_q, hd, dev)
-    if q.dtype is not dt or out.dtype is not dt:
-        raise MoeError(MOE_ERR_INVALID, "q and out: the cache's type is wanted")
-    n_seq, mp = block_table.shape
-    wp, wn = None, 0
-    if workspace is not None:
-        if not workspace.is_contiguous() or workspace.get_device() != dev:
-            raise MoeError(MOE_ERR_INVALID, f"workspace: a contiguous tensor on cuda:{dev} is wanted")
-        wp, wn = workspace.data_ptr(), workspace.nbytes
-    check(lib().moe_paged_attention_dev(
-        qp, ldq, c, _dev(block_table, i32, n_seq * mp, "block_table", dev), n_seq, mp,
-        _dev(row_seq, i32, rows, "row_seq", dev), _dev(row_pos, i32, rows, "row_pos", dev), rows, n_q, max_kv, scale,
-        op, ldo, _dev(lse, _Types.f32, rows * n_q, "lse", dev), wp, wn, _stream(stream)))
-
-
-def route(logits, topk_idx, topk_p, bias=None, score="softmax", groups=1, keep_groups=1, group_top=1, renorm=True,
-          scale=1.0, stream=None):
-    """moe_route_dev: topk_idx (int32) and topk_p (fp32) [rows][top_k] of
-    logits [rows][E] (rows may lie apart)."""
-    dev, dt = _cuda_device(logits, "route"), _elem(logits, "logits")
-    (T, E), st = logits.shape, logits.stride()
-    if st[1] != 1 and T and E > 1:
-        raise MoeError(MOE_ERR_INVALID, "logits: the experts must be contiguous")
-    kind = ROUTE_SCORES.get(score)
-    if kind is None:
-        raise MoeError(MOE_ERR_INVALID, f"score: one of {sorted(ROUTE_SCORES)} is wanted")
-    k = topk_idx.shape[1]
-    check(lib().moe_route_dev(
-        logits.data_ptr(), st[0] if T > 1 else E, dt, T, E, _dev(bias, _Types.f32, E, "bias", dev), kind, groups,
-        keep_groups, group_top, k, 1 if renorm else 0, scale, _dev(topk_idx, _Types.i32, T * k, "topk_idx", dev),
-        _dev(topk_p, _Types.f32, T * k, "topk_p", dev), _stream(stream)))
+    return lib().moe_paged_attention_workspace(rows, n_q, C.byref(kv_cache(k_cache, v_cache)), max_kv)
 
 
 def profile(enable):

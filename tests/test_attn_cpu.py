@@ -138,6 +138,27 @@ def test_binding_refuses_host_tensors_and_wrong_types():
             call()
 
 
+def test_binding_arguments():
+    """Positions and keywords as documented; unknown, double and missing ones are a TypeError, as of a Python function."""
+    torch = pytest.importorskip("torch")
+    for f in (mc.kv_plan, mc.qk_norm_rope, mc.paged_attention, mc.route):
+        assert f.__doc__ and f.__name__ in f.__doc__
+        with pytest.raises(TypeError):
+            f()
+        with pytest.raises(TypeError):
+            f(*range(20))
+    x, i, p = torch.zeros(2, 8), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2)
+    with pytest.raises(TypeError):
+        mc.route(x, i, p, experts=3)
+    with pytest.raises(TypeError):
+        mc.route(x, i, p, topk_p=p)
+    for bad in ((None, i, p), (3, i, p), (x, "i", p), (x.double(), i, p), (x, i.long(), p)):
+        with pytest.raises(mc.MoeError) as e:
+            mc.route(*bad)
+        assert e.value.code == INVALID
+    assert not hasattr(mc, "no_such_call")
+
+
 def test_page_division_by_multiplication():
     """The kernels divide positions by the page size with one multiply; the
     same arithmetic here, at the quotients' edges, for every page size that

@@ -72,7 +72,7 @@ struct MhModel {
      + b of a layer for pages j of sequence b; the plan of the rows at
      (plan_pos, plan_T); staging of the projected rows */
   int kv_dtype, kv_page, kv_max_pages, plan_pos, plan_T, plan_cap, kv_cap;
-  int kv_on;
+  int kv_on, kv_device;            /* and the device that holds them */
   void *d_kc, *d_vc;
   float* d_rope;                 /* [max_ctx][head_dim]: cosines, sines */
   int *d_table, *d_free, *d_len, *d_rows;
@@ -556,6 +556,19 @@ static int kv_plan(MhModel* m, int pos, int T) {
   return MOE_OK;
 }
 
+/* The caches' device becomes the calling thread's; returns the one to go back to. */
+static int kv_enter(const MhModel* m) {
+  int cur = m->kv_device;
+  cudaGetDevice(&cur);
+  if (cur != m->kv_device) cudaSetDevice(m->kv_device);
+  return cur;
+}
+static int kv_leave(const MhModel* m, int back, int rc) {
+  if (rc) cudaStreamSynchronize(m->kv_stream);   /* nothing of a failed call is left in flight */
+  if (back != m->kv_device) cudaSetDevice(back);
+  return rc;
+}
+
 /* q, k, v of the new rows (in h_qkv) -> norm, rotation, append, attention ->
    m->hcat, for layer l at the current position. */
 static int kv_attention(MhModel* m, int l, int T) {
@@ -615,6 +628,8 @@ int mh_kv_device(MhModel* m, int dtype, int page_size) {
   if (max_pages * m->batch * page_size > 0x7fffffffll)
     return fail(MOE_ERR_UNSUPPORTED, "mh_kv_device: more than 2^31 - 1 positions a layer");
   if (m->kv_on) free_kv(m);
+  m->kv_device = 0;
+  cudaGetDevice(&m->kv_device);
   m->kv_on = 1;                    /* what is allocated below goes with the model */
   m->kv_dtype = dtype;
   m->kv_page = page_size;
@@ -670,7 +685,8 @@ int mh_attention(MhModel* m, int layer, const float* x, int T, float* x_after, f
 
   float *q = m->q, *k = m->k, *v = m->v;
   if (m->kv_on) {                  /* straight into the page-locked staging */
-    if ((rc = kv_rows(m, R))) return rc;
+    const int back = kv_enter(m);
+    if ((rc = kv_leave(m, back, kv_rows(m, R)))) return rc;
     q = m->h_qkv; k = q + (size_t)R * Dq; v = k + (size_t)R * Dkv;
   }
   rmsnorm_rows(x, w->rms1_w, R, D, eps, m->xn1);
@@ -683,7 +699,8 @@ int mh_attention(MhModel* m, int layer, const float* x, int T, float* x_after, f
     if (w->bv) for (int i = 0; i < Dkv; ++i) v[(size_t)r * Dkv + i] += w->bv[i];
   }
   if (m->kv_on) {
-    if ((rc = kv_attention(m, layer, T))) return rc;
+    const int back = kv_enter(m);
+    if ((rc = kv_leave(m, back, kv_attention(m, layer, T)))) return rc;
     goto out_product;
   }
 #pragma omp parallel for schedule(static)
@@ -1165,7 +1182,10 @@ int mh_fill_kv(MhModel* m, int ctx, uint64_t seed, float std) {
   const size_t row = (size_t)ctx * m->Dkv;           /* one (layer, sequence) block */
   float* tmp = NULL;
   if (row == 0) { m->pos = ctx; return MOE_OK; }
-  if (m->kv_on) return kv_fill(m, ctx, seed, std);
+  if (m->kv_on) {
+    const int back = kv_enter(m);
+    return kv_leave(m, back, kv_fill(m, ctx, seed, std));
+  }
   CUDA_OK(cudaMalloc((void**)&tmp, sizeof(float) * row), "device staging");
   for (int l = 0; l < m->c.n_layers; ++l)
     for (int b = 0; b < m->batch; ++b)

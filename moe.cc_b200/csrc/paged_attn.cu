@@ -668,7 +668,7 @@ __device__ __forceinline__ void clear_heads(const AttnArgs& a, int row, int head
     for (int h = threadIdx.x; h < heads; h += blockDim.x) a.lse[(long long)row * a.n_q + head0 + h] = -INFINITY;
 }
 
-// How the work is split, a "item" being a row's key-value head and tile:
+// How the work is split, an "item" being a row's key-value head and tile:
 //   kDealt      The CTAs are taken in groups, one for each key-value head (and
 //               tile), and the pieces of all rows, one row after another, are
 //               cut into as many stretches, equal to a piece, as there are

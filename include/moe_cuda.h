@@ -408,8 +408,9 @@ int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k, long long 
  * (test_model_trace.c:394-420); query head h reads key-value head
  * h / (n_q / n_kv). row_seq[i] is row i's row of block_table[n_seq][max_pages]
  * (NULL: row i of the table). q and out have the cache's type, ldq and ldo
- * elements from row to row; out may be q (same stride). lse [rows][n_q]
- * (NULL to skip): the natural logarithm of the softmax's sum, scale included.
+ * elements from row to row; out may be q (same stride) and must not overlap it
+ * otherwise. lse [rows][n_q] (NULL to skip): the natural logarithm of the
+ * softmax's sum, scale included.
  *   - row_seq outside [0, n_seq): padding, the row of out and lse stays as it is.
  *   - row_pos negative: no position; out is 0, lse -inf (also when every score
  *     is -inf).

@@ -90,6 +90,19 @@ inline int check_cache(const MoeKvCache* c, const char* who) {
   return MOE_OK;
 }
 
+// whether `rows` rows of two operands, n elements of e bytes each and ld from
+// one to the next, may share a byte: their ranges meet, and they are not
+// columns of one matrix that lie beside each other
+inline bool overlap(const void* p, long long ldp, long long np, int ep, const void* r, long long ldr, long long nr,
+                    int er, int rows) {
+  const long long p0 = (long long)(uintptr_t)p, r0 = (long long)(uintptr_t)r, sp = ldp * ep, sr = ldr * er;
+  const long long bp = np * ep, br = nr * er;
+  if (p0 + (rows - 1) * sp + bp <= r0 || r0 + (rows - 1) * sr + br <= p0) return false;
+  if (sp != sr || sp <= 0) return true;
+  const long long d = ((r0 - p0) % sp + sp) % sp;       // from a row of p to the next row of r
+  return d < bp || d + br > sp;
+}
+
 // n / d for 0 <= n < 2^31 by one multiply: with l = ceil(log2 d) and
 // m = floor(2^(31+l) / d) + 1, the excess e = m d - 2^(31+l) lies in (0, d],
 // so e n < 2^(31+l) and floor(n m / 2^(31+l)) = floor(n / d).

@@ -991,6 +991,9 @@ extern "C" int moe_paged_attention_dev(const void* q, long long ldq, const MoeKv
     return at::fail(MOE_ERR_INVALID, "%s: rows of q or out overlap", who);
   if ((uintptr_t)q % 16 || (uintptr_t)out % 16 || ldq % (16 / es) || ldo % (16 / es))
     return at::fail(MOE_ERR_INVALID, "%s: rows of q and out must start on 16-byte boundaries", who);
+  const long long nq = (long long)n_q * hd;
+  if (!(out == q && ldo == ldq) && at::overlap(out, ldo, nq, es, q, ldq, nq, es, rows))
+    return at::fail(MOE_ERR_INVALID, "%s: out overlaps q without being q", who);
   const int group = n_q / cache->n_kv, ht = head_tile(cache->dtype, hd, group);
   AttnArgs a{};
   a.tiles = (group + ht - 1) / ht;

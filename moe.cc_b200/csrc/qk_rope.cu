@@ -249,15 +249,6 @@ cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
   return go(qk_norm_rope_kernel<TI, TO, 4, 32, false>, 32);
 }
 
-// whether the row-strided ranges [p, p + ((rows-1) ld + n) es) of two
-// operands share a byte
-bool overlap(const void* p, long long ldp, long long np, int ep, const void* r, long long ldr, long long nr, int er,
-             int rows) {
-  const uintptr_t p0 = (uintptr_t)p, p1 = p0 + (uintptr_t)(((rows - 1) * ldp + np) * ep);
-  const uintptr_t r0 = (uintptr_t)r, r1 = r0 + (uintptr_t)(((rows - 1) * ldr + nr) * er);
-  return p0 < r1 && r0 < p1;
-}
-
 }  // namespace
 }  // namespace moe
 
@@ -297,10 +288,10 @@ extern "C" int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k,
   // q_out may be q itself; any other overlap would be read after it was written
   const long long nq = (long long)n_q * hd, nk = (long long)cache->n_kv * hd;
   const bool same = q_out == q && ldo == ldq && es == eo;
-  if (n_q && !same && overlap(q_out, ldo, nq, eo, q, ldq, nq, es, rows))
+  if (n_q && !same && at::overlap(q_out, ldo, nq, eo, q, ldq, nq, es, rows))
     return at::fail(MOE_ERR_INVALID, "%s: q_out overlaps q without being q", who);
   if (n_q && !same && row_slot &&
-      (overlap(q_out, ldo, nq, eo, k, ldk, nk, es, rows) || overlap(q_out, ldo, nq, eo, v, ldv, nk, es, rows)))
+      (at::overlap(q_out, ldo, nq, eo, k, ldk, nk, es, rows) || at::overlap(q_out, ldo, nq, eo, v, ldv, nk, es, rows)))
     return at::fail(MOE_ERR_INVALID, "%s: q_out overlaps k or v", who);
   at::OnDeviceOf on;
   if ((rc = on.enter(n_q ? q : k, who))) return rc;

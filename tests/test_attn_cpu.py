@@ -91,6 +91,14 @@ def test_rope_refuses(over, want):
     assert rope(**over) == want
 
 
+@pytest.mark.parametrize("over", [
+    dict(out=P + 512), dict(out=P, ldo=512), dict(out=P + 1024, ldq=512, ldo=512 + 64), dict(ldq=480, out=P + 512, ldo=480)])
+def test_attention_refuses_an_output_across_its_queries(over):
+    """Rows of 512 bytes: another offset, another stride, columns that meet at
+    either end."""
+    assert attn(**over) == INVALID and b"overlaps q" in mc.lib().moe_cuda_last_error()
+
+
 @pytest.mark.parametrize("over,want", [
     (dict(rows=-1), INVALID), (dict(n_q=3), INVALID), (dict(n_q=0), INVALID), (dict(n_q=32770), UNSUPPORTED), (dict(n_seq=-1), INVALID),
     (dict(max_pages=0), INVALID), (dict(rows=5), INVALID), (dict(max_kv=0), INVALID), (dict(q=None), INVALID),

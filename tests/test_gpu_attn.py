@@ -451,6 +451,30 @@ def test_norm_rope_append(gpu, ti, to, n_q, n_kv, hd, rot, ps, rows, norm):
     assert torch.equal(k2, kc) and torch.equal(v2, vc)
 
 
+def test_outputs_beside_their_inputs_in_one_matrix(gpu):
+    """Inputs and outputs that are columns of one matrix do not overlap: the
+    same bits as apart, and the other columns stay."""
+    R, nq, nk, hd, ps = 7, 4, 2, 64, 16
+    q, kc, vc, table = make_attn(torch.bfloat16, R, nq, nk, hd, ps, [40, 1, 5000, 64, 16, 700, 3], seed=21)
+    pos = torch.tensor([39, 0, 4999, 63, 15, 699, 2], dtype=torch.int32, device="cuda")
+    n, m = nq * hd, nk * hd
+    x = torch.randn(R, n + 2 * m + 2 * n + 8, device="cuda").bfloat16()
+    col = lambda t, a, h: t[:, a:a + h * hd].unflatten(1, (h, hd))
+    ins = lambda t: (col(t, n, nq), col(t, 2 * n, nk), col(t, 2 * n + m, nk))      # q_out, q, k, v, attention's out
+    rope = rope_table(5000, hd)
+    slot = torch.arange(R, dtype=torch.int32, device="cuda")
+    apart, kr, vr = torch.empty(R, nq, hd, device="cuda", dtype=torch.bfloat16), torch.zeros_like(kc), torch.zeros_like(vc)
+    mc.qk_norm_rope(*ins(x), kr, vr, pos, slot, apart, rope=rope)
+    y, k2, v2 = x.clone(), torch.zeros_like(kc), torch.zeros_like(vc)
+    mc.qk_norm_rope(*ins(y), k2, v2, pos, slot, col(y, 0, nq), rope=rope)
+    assert torch.equal(col(y, 0, nq), apart) and torch.equal(y[:, n:], x[:, n:])
+    assert torch.equal(k2, kr) and torch.equal(v2, vr)
+    want, _ = run_attn(apart, kc, vc, table, pos, 0.1, 5000)
+    run_attn(col(y, 0, nq), kc, vc, table, pos, 0.1, 5000, out=col(y, 2 * n + 2 * m, nq))
+    assert torch.equal(col(y, 2 * n + 2 * m, nq), want) and torch.equal(col(y, 0, nq), apart)
+    assert torch.equal(y[:, n:2 * n + 2 * m], x[:, n:2 * n + 2 * m]) and torch.equal(y[:, -8:], x[:, -8:])
+
+
 def test_append_without_rotation_copies(gpu):
     """rot_dim 0 and no norm: the rows arrive unchanged, whatever they hold."""
     kv = torch.tensor([NAN, math.inf, -math.inf, -0.0, 1e-40, 65504.0, 1.0, 2.0], device="cuda").repeat(6, 1, 1)

@@ -441,8 +441,10 @@ int moe_paged_attention_dev(const void* q, long long ldq, const MoeKvCache* cach
  * index. n_group > 1: of the n_group equal groups of consecutive experts, only
  * the keep_group with the largest sum of their best group_top (1 or 2) values
  * are chosen from. The weight is s, without the bias, divided by the sum of
- * the chosen (renorm != 0), times factor, in fp32. The choice is the one that
- * scores in 64 bits make (they are computed where fp32 cannot tell). An expert
+ * the chosen (renorm != 0), times factor, in fp32. Groups, and with a bias the
+ * experts, are chosen as scores in 64 bits choose them (they are computed where
+ * fp32 cannot tell); without a bias experts go by their logits, which order
+ * the exact scores also where those have become one number. An expert
  * whose logit is NaN or -inf, or whose bias is, is never chosen; where fewer
  * than top_k are left, the index is -1 and the weight 0.
  * E up to 1024, n_group and top_k up to 32. Device pointers, asynchronous, no

@@ -12,13 +12,15 @@
 // The choice is an ordering, and it is the order of the exact scores that is
 // wanted: in fp32 two different sigmoid scores near 1 (or scores plus a bias)
 // round to the same number often enough to change which expert is chosen.
-// Without a bias or groups the order of the scores is the order of the logits,
-// exactly, and no score is needed for it. Otherwise a token is first ranked by
-// fp32 scores, whose error is bounded (`margin`): the list of the best goes on
-// past top_k until the next is clearly behind, and if two neighbours in it are
-// closer than the bound, its few experts are ordered again by scores in 64 bits.
-// Where the groups on either side of the cut are that close, the whole token is
-// ranked again in 64 bits. The weights are fp32 softmax or sigmoid values.
+// Without a bias the order of the scores is the order of the logits, exactly,
+// and the experts (with groups: those of the groups that stay) are taken by
+// logit. (Scores, even in 64 bits, would not do: the sigmoid is 1 from 37 on.)
+// With a bias a token is first ranked by fp32 choices, whose error is bounded
+// (`margin`): the list of the best goes on past top_k until the next is clearly
+// behind, and if two neighbours in it are closer than the bound, its few experts
+// are ordered again by choices in 64 bits. Groups are chosen by fp32 sums too,
+// and where two on either side of the cut are that close, by sums in 64 bits.
+// The weights are fp32 softmax or sigmoid values.
 //
 // One warp routes one token: expert j * 32 + lane in lane `lane`. A round of
 // the selection takes the largest key by a warp reduction, then the lowest
@@ -265,13 +267,13 @@ __device__ __noinline__ int choose64(const RouteArgs& a, const float (&x)[EPL], 
   return chosen;
 }
 
-// The n experts that lanes 0 .. n - 1 list, in the order of their choices in
-// 64 bits; lane r returns the r-th.
+// With a bias: the n experts that lanes 0 .. n - 1 list, in the order of their
+// choices in 64 bits; lane r returns the r-th.
 template <typename T, int EPL>
 __device__ __noinline__ int order64(const RouteArgs& a, const float (&x)[EPL], float top, long long t, int listed, int n) {
   const int lane = threadIdx.x & 31;
   double total = 1.0;
-  if (a.softmax && a.bias) {                    // without a bias the sum orders nothing
+  if (a.softmax) {
     total = 0.0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) total += x[j] > -INFINITY ? soft64(x[j], top) : 0.0;
@@ -280,8 +282,7 @@ __device__ __noinline__ int order64(const RouteArgs& a, const float (&x)[EPL], f
   double c = 0.0;
   if (lane < n) {
     const float xe = logit<T>(a.x, t * a.ld + listed);
-    c = a.softmax ? soft64(xe, top) / total : sigm64(xe);
-    if (a.bias) c += (double)a.bias[listed];
+    c = (a.softmax ? soft64(xe, top) / total : sigm64(xe)) + (double)a.bias[listed];
   }
   int rank = 0;
   for (int m = 0; m < n; ++m) {
@@ -297,8 +298,49 @@ __device__ __noinline__ int order64(const RouteArgs& a, const float (&x)[EPL], f
   return chosen;
 }
 
-// EPL experts a lane; SCORED: the choice needs every score (bias or groups)
-template <typename T, int EPL, bool SCORED>
+// The experts that stay, by logit; lane r returns the r-th.
+template <typename T, int EPL>
+__device__ __forceinline__ int choose_by_logit(const RouteArgs& a, const float (&x)[EPL], unsigned stays) {
+  const int lane = threadIdx.x & 31;
+  unsigned key[EPL];
+  int chosen = -1;
+  if constexpr (sizeof(T) == 2) {
+    // the logit's 16 bits above, the index from the top down below them
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      const unsigned e = j * 32 + lane;
+      unsigned b;
+      if constexpr (std::is_same<T, __half>::value) b = __half_as_ushort(__float2half_rn(x[j] + 0.0f));
+      else b = __float_as_uint(x[j] + 0.0f) >> 16;
+      b = (b ^ (b >> 15 ? 0xffffu : 0x8000u)) & 0xffffu;
+      key[j] = x[j] > -INFINITY && (stays == ~0u || stays_in(a, stays, j)) ? b << 16 | (0xffffu - e) : 0u;
+    }
+    sort_keys<EPL>(key);
+    unsigned mine = 0u;
+    for (int r = 0; r < a.topk; ++r) {
+      const unsigned best = pop<EPL>(key);
+      if (best == 0u) break;
+      if (lane == r) mine = best;
+    }
+    chosen = mine ? 0xffff - (int)(mine & 0xffffu) : -1;
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      key[j] = x[j] > -INFINITY && (stays == ~0u || stays_in(a, stays, j)) ? key_of(x[j]) : 0u;
+    for (int r = 0; r < a.topk; ++r) {
+      unsigned k;
+      const int e = take<EPL>(key, k);
+      if (e < 0) break;
+      if (lane == r) chosen = e;
+    }
+  }
+  return chosen;
+}
+
+// EPL experts a lane. MODE: what the choice needs: logits alone; every score for
+// the groups, then logits; every score and the bias.
+enum { kByLogit, kByGroup, kByScore };
+template <typename T, int EPL, int MODE>
 __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteArgs a) {
   extern __shared__ double choice_sm[];                    // groups: [kWarps][EPL * 32]
   pdl_wait();
@@ -307,7 +349,6 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
   const long long t = (long long)blockIdx.x * kWarps + warp;
   if (t >= a.rows) return;
   float x[EPL];
-  unsigned key[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = j * 32 + lane;
@@ -316,7 +357,7 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
   }
   float top = -INFINITY;
   int chosen = -1;                                         // lane r: the r-th choice
-  if constexpr (SCORED) {
+  if constexpr (MODE != kByLogit) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
     const unsigned tk = __reduce_max_sync(~0u, key_of(top));
@@ -329,78 +370,58 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
       float cut[2];
       stays = best_groups<float, EPL>(a, (float*)mine, c, cut);
       if (cut[0] - cut[1] < 2 * margin(a, cut[0], cut[1], 0.f)) stays = best_groups64<EPL>(a, x, top, mine);
+      if constexpr (MODE == kByScore)
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (!stays_in(a, stays, j)) c[j] = -INFINITY;
+    }
+    if constexpr (MODE == kByGroup) {
+      chosen = choose_by_logit<T, EPL>(a, x, stays);
+    } else {
+      // Keys: the fp32 choice without its lowest bits, which hold the index from
+      // the top down. Lane n keeps the n-th; top_k + 1 of them, and on until the
+      // next one is clearly behind the one before: nothing outside the list can
+      // then belong in its first top_k.
+      constexpr unsigned kLow = EPL * 32 - 1;
+      constexpr float kDrop = (float)(EPL * 32) * 0x1p-23f;
+      unsigned key[EPL];
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
-        if (!stays_in(a, stays, j)) c[j] = -INFINITY;
+        key[j] = c[j] > -INFINITY ? (key_of(c[j]) & ~kLow) | (kLow - (j * 32 + lane)) : 0u;
+      sort_keys<EPL>(key);
+      unsigned mine = 0u;
+      int n = 0;
+      for (; n < min(a.topk + 1, 32); ++n) {
+        const unsigned best = pop<EPL>(key);
+        if (best == 0u) break;
+        if (lane == n) mine = best;
+      }
+      auto near = [&]() -> unsigned {                        // bit i: entry i + 1 is not clearly behind entry i
+        const float u = value_of(mine & ~kLow), v = __shfl_down_sync(~0u, u, 1);
+        return __ballot_sync(~0u, lane + 1 < n && !(u - v >= margin(a, u, v, kDrop)));
+      };
+      unsigned close = near();
+      bool anew = false;
+      while (n > a.topk && (close >> (n - 2)) & 1) {         // the last is not: the list goes on
+        const unsigned best = pop<EPL>(key);
+        if (best == 0u) break;
+        if (n == 32) { anew = true; break; }
+        if (lane == n) mine = best;
+        ++n;
+        close = near();
+      }
+      if (a.topk == 32 && !anew) {                           // no lane is left to look behind the last
+        const unsigned best = pop<EPL>(key);
+        const float u = __shfl_sync(~0u, value_of(mine & ~kLow), 31), v = value_of(best & ~kLow);
+        anew = best != 0u && !(u - v >= margin(a, u, v, kDrop));
+      }
+      chosen = mine ? (int)(kLow - (mine & kLow)) : -1;
+      if (anew) chosen = choose64<EPL>(a, x, top, stays);
+      else if (close) chosen = order64<T, EPL>(a, x, top, t, chosen, __popc(__ballot_sync(~0u, mine != 0u)));
+      if (lane >= a.topk) chosen = -1;
     }
-    // Keys: the fp32 choice without its lowest bits, which hold the index from
-    // the top down. Lane n keeps the n-th; top_k + 1 of them, and on until the
-    // next one is clearly behind the one before: nothing outside the list can
-    // then belong in its first top_k.
-    constexpr unsigned kLow = EPL * 32 - 1;
-    constexpr float kDrop = (float)(EPL * 32) * 0x1p-23f;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      key[j] = c[j] > -INFINITY ? (key_of(c[j]) & ~kLow) | (kLow - (j * 32 + lane)) : 0u;
-    sort_keys<EPL>(key);
-    unsigned mine = 0u;
-    int n = 0;
-    for (; n < min(a.topk + 1, 32); ++n) {
-      const unsigned best = pop<EPL>(key);
-      if (best == 0u) break;
-      if (lane == n) mine = best;
-    }
-    auto near = [&]() -> unsigned {                        // bit i: entry i + 1 is not clearly behind entry i
-      const float u = value_of(mine & ~kLow), v = __shfl_down_sync(~0u, u, 1);
-      return __ballot_sync(~0u, lane + 1 < n && !(u - v >= margin(a, u, v, kDrop)));
-    };
-    unsigned close = near();
-    bool anew = false;
-    while (n > a.topk && (close >> (n - 2)) & 1) {         // the last is not: the list goes on
-      const unsigned best = pop<EPL>(key);
-      if (best == 0u) break;
-      if (n == 32) { anew = true; break; }
-      if (lane == n) mine = best;
-      ++n;
-      close = near();
-    }
-    if (a.topk == 32 && !anew) {                           // no lane is left to look behind the last
-      const unsigned best = pop<EPL>(key);
-      const float u = __shfl_sync(~0u, value_of(mine & ~kLow), 31), v = value_of(best & ~kLow);
-      anew = best != 0u && !(u - v >= margin(a, u, v, kDrop));
-    }
-    chosen = mine ? (int)(kLow - (mine & kLow)) : -1;
-    if (anew) chosen = choose64<EPL>(a, x, top, stays);
-    else if (close) chosen = order64<T, EPL>(a, x, top, t, chosen, __popc(__ballot_sync(~0u, mine != 0u)));
-    if (lane >= a.topk) chosen = -1;
-  } else if constexpr (sizeof(T) == 2) {
-    // the logit's 16 bits above, the index from the top down below them
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const unsigned e = j * 32 + lane;
-      unsigned b;
-      if constexpr (std::is_same<T, __half>::value) b = __half_as_ushort(__float2half_rn(x[j] + 0.0f));
-      else b = __float_as_uint(x[j] + 0.0f) >> 16;
-      b = (b ^ (b >> 15 ? 0xffffu : 0x8000u)) & 0xffffu;
-      key[j] = x[j] > -INFINITY ? b << 16 | (0xffffu - e) : 0u;
-    }
-    sort_keys<EPL>(key);
-    unsigned mine = 0u;
-    for (int r = 0; r < a.topk; ++r) {
-      const unsigned best = pop<EPL>(key);
-      if (best == 0u) break;
-      if (lane == r) mine = best;
-    }
-    chosen = mine ? 0xffff - (int)(mine & 0xffffu) : -1;
   } else {
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) key[j] = x[j] > -INFINITY ? key_of(x[j]) : 0u;
-    for (int r = 0; r < a.topk; ++r) {
-      unsigned k;
-      const int e = take<EPL>(key, k);
-      if (e < 0) break;
-      if (lane == r) chosen = e;
-    }
+    chosen = choose_by_logit<T, EPL>(a, x, ~0u);
   }
 
   const float xe = chosen >= 0 ? logit<T>(a.x, t * a.ld + chosen) : 0.f;
@@ -415,7 +436,7 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
     const float sum = warp_sum_of(s);
     s = sum > 0.f ? s / sum : 0.f;
   } else if (a.softmax) {
-    if constexpr (!SCORED) top = __shfl_sync(~0u, xe, 0);  // the first choice is the largest logit
+    if constexpr (MODE == kByLogit) top = __shfl_sync(~0u, xe, 0);  // the first choice is the largest logit
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) sum += x[j] > -INFINITY ? soft(x[j], top) : 0.f;
@@ -431,22 +452,23 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
 }
 
 template <typename T, int EPL>
-cudaError_t launch_route_epl(const RouteArgs& a, bool scored, cudaStream_t st) {
+cudaError_t launch_route_epl(const RouteArgs& a, cudaStream_t st) {
   const unsigned grid = (unsigned)((a.rows + kWarps - 1) / kWarps);
   const size_t smem = a.groups > 1 ? sizeof(double) * kWarps * EPL * 32 : 0;
-  if (scored) return launch_pdl(expert_route_kernel<T, EPL, true>, dim3(grid), dim3(kWarps * 32), smem, st, a);
-  return launch_pdl(expert_route_kernel<T, EPL, false>, dim3(grid), dim3(kWarps * 32), 0, st, a);
+  if (a.bias) return launch_pdl(expert_route_kernel<T, EPL, kByScore>, dim3(grid), dim3(kWarps * 32), smem, st, a);
+  if (a.groups > 1) return launch_pdl(expert_route_kernel<T, EPL, kByGroup>, dim3(grid), dim3(kWarps * 32), smem, st, a);
+  return launch_pdl(expert_route_kernel<T, EPL, kByLogit>, dim3(grid), dim3(kWarps * 32), 0, st, a);
 }
 
 template <typename T>
-cudaError_t launch_route(const RouteArgs& a, bool scored, cudaStream_t st) {
+cudaError_t launch_route(const RouteArgs& a, cudaStream_t st) {
   const int epl = (a.E + 31) / 32;
-  if (epl <= 1) return launch_route_epl<T, 1>(a, scored, st);
-  if (epl <= 2) return launch_route_epl<T, 2>(a, scored, st);
-  if (epl <= 4) return launch_route_epl<T, 4>(a, scored, st);
-  if (epl <= 8) return launch_route_epl<T, 8>(a, scored, st);
-  if (epl <= 16) return launch_route_epl<T, 16>(a, scored, st);
-  return launch_route_epl<T, 32>(a, scored, st);
+  if (epl <= 1) return launch_route_epl<T, 1>(a, st);
+  if (epl <= 2) return launch_route_epl<T, 2>(a, st);
+  if (epl <= 4) return launch_route_epl<T, 4>(a, st);
+  if (epl <= 8) return launch_route_epl<T, 8>(a, st);
+  if (epl <= 16) return launch_route_epl<T, 16>(a, st);
+  return launch_route_epl<T, 32>(a, st);
 }
 
 }  // namespace
@@ -481,9 +503,8 @@ extern "C" int moe_route_dev(const void* logits, long long ld, int dtype, int ro
   a.group = at::FastDiv((unsigned)(E / n_group));
   a.lanes_per_group = 1;
   while (2 * a.lanes_per_group * n_group <= 32) a.lanes_per_group *= 2;
-  const bool scored = bias || a.groups > 1;
   cudaStream_t st = (cudaStream_t)stream;
-  return at::launched(dtype == MOE_DTYPE_F32    ? launch_route<float>(a, scored, st)
-                      : dtype == MOE_DTYPE_BF16 ? launch_route<__nv_bfloat16>(a, scored, st)
-                                                : launch_route<__half>(a, scored, st), who);
+  return at::launched(dtype == MOE_DTYPE_F32    ? launch_route<float>(a, st)
+                      : dtype == MOE_DTYPE_BF16 ? launch_route<__nv_bfloat16>(a, st)
+                                                : launch_route<__half>(a, st), who);
 }

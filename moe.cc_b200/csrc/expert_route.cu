@@ -19,7 +19,7 @@
 // (`margin`): the list of the best goes on past top_k until the next is clearly
 // behind, and if two neighbours in it are closer than the bound, its few experts
 // are ordered again by choices in 64 bits. Groups are chosen by fp32 sums too,
-// and where two on either side of the cut are that close, by sums in 64 bits.
+// and where their bounds meet across the cut, by sums in 64 bits.
 // The weights are fp32 softmax or sigmoid values.
 //
 // One warp routes one token: expert j * 32 + lane in lane `lane`. A round of
@@ -134,10 +134,13 @@ __device__ __forceinline__ float margin(const RouteArgs& a, float u, float v, fl
   return fmaf(m, drop, (a.softmax ? 0x1p-17f : 0x1p-20f) * (1.0f + m));
 }
 
-// Which of the groups stay, a bit at lane (group * lanes_per_group). cut[0],
-// cut[1]: the least sum that stays and the largest that does not.
+// Which of the groups stay, a bit at lane (group * lanes_per_group). sure (fp32):
+// whether 64-bit sums choose the same. A group's sum errs by no more than the
+// margin of its two addends (which may be large and cancel; the sum's own
+// rounding is below what the margin has to spare), so it is sure where no
+// group that stays may lie below one that does not.
 template <typename F, int EPL>
-__device__ __forceinline__ unsigned best_groups(const RouteArgs& a, F* mine, const F (&c)[EPL], F (&cut)[2]) {
+__device__ __forceinline__ unsigned best_groups(const RouteArgs& a, F* mine, const F (&c)[EPL], bool& sure) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
 #pragma unroll
@@ -157,25 +160,30 @@ __device__ __forceinline__ unsigned best_groups(const RouteArgs& a, F* mine, con
     b1 = max(min(b0, o0), max(b1, o1));
     b0 = max(b0, o0);
   }
-  const F gs = b0 + (a.group_top == 2 && b1 > -INFINITY ? b1 : (F)0);
+  const F second = a.group_top == 2 && b1 > -INFINITY ? b1 : (F)0, gs = b0 + second;
   // a group stays if fewer than `keep` groups come before it
   int before = 0;
   for (int h = 0; h < a.groups; ++h) {
     const F v = __shfl_sync(~0u, gs, h * lpg);
     before += v > gs || (v == gs && h < grp);
   }
-  const bool head = grp < a.groups && lane % lpg == 0;
-  cut[0] = __shfl_sync(~0u, gs, __ffs(__ballot_sync(~0u, head && before == a.keep - 1)) - 1);
-  cut[1] = __shfl_sync(~0u, gs, __ffs(__ballot_sync(~0u, head && before == a.keep)) - 1);
-  return __ballot_sync(~0u, head && before < a.keep);
+  const bool head = grp < a.groups && lane % lpg == 0, stays = head && before < a.keep;
+  if constexpr (sizeof(F) == 4) {
+    const float e = b0 > -INFINITY ? margin(a, b0, second, 0.f) : 0.f;     // a group without experts is exact
+    const unsigned least = __reduce_min_sync(~0u, stays ? key_of(gs - e) : ~0u);
+    const unsigned most = __reduce_max_sync(~0u, head && !stays ? key_of(gs + e) : 0u);
+    sure = !__any_sync(~0u, head && !(e < INFINITY)) && least >= most;
+  }
+  return __ballot_sync(~0u, stays);
 }
 
 // The same by choices in 64 bits.
 template <int EPL>
 __device__ __noinline__ unsigned best_groups64(const RouteArgs& a, const float (&x)[EPL], float top, double* mine) {
-  double c[EPL], cut[2];
+  double c[EPL];
+  bool sure;
   choices<double, EPL>(a, x, top, c);
-  return best_groups<double, EPL>(a, mine, c, cut);
+  return best_groups<double, EPL>(a, mine, c, sure);
 }
 
 // Whether expert j * 32 + lane is in a group that stays.
@@ -367,9 +375,9 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
     unsigned stays = ~0u;
     if (a.groups > 1) {
       double* mine = choice_sm + warp * (EPL * 32);
-      float cut[2];
-      stays = best_groups<float, EPL>(a, (float*)mine, c, cut);
-      if (cut[0] - cut[1] < 2 * margin(a, cut[0], cut[1], 0.f)) stays = best_groups64<EPL>(a, x, top, mine);
+      bool sure;
+      stays = best_groups<float, EPL>(a, (float*)mine, c, sure);
+      if (!sure) stays = best_groups64<EPL>(a, x, top, mine);
       if constexpr (MODE == kByScore)
 #pragma unroll
         for (int j = 0; j < EPL; ++j)

@@ -414,6 +414,10 @@ int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k, long long 
  *   - row_seq outside [0, n_seq): padding, the row of out and lse stays as it is.
  *   - row_pos negative: no position; out is 0, lse -inf (also when every score
  *     is -inf).
+ *   - Infinities and NaN in attended keys and values enter as in fp32
+ *     arithmetic: a score of -inf has weight 0, one of +inf or NaN makes the
+ *     row's key-value head NaN, an infinite value gives infinite outputs. (A
+ *     run of positions that meets one is computed twice: right, but slower.)
  *   - Positions past max_pages * page_size and positions on a page outside
  *     [0, n_pages) are not attended. Slots past row_pos are never read,
  *     whatever they hold.

@@ -34,6 +34,10 @@
 // rounding does. With an fp32 cache both products run as three tf32 products
 // of high and low parts (the low parts' product, 2^-24, is left out), summed
 // from zero per step and added to fp32 sums outside the tensor core.
+//
+// An operand in two parts is not what it was where it is infinite (inf - inf is
+// no remainder, and inf times a remainder of 0 is NaN). A warp whose sums come
+// out NaN therefore takes its run again with plain fp32 products (attend, "NaN").
 #include "attn.cuh"
 
 #include <float.h>
@@ -124,8 +128,8 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], const unsigned (&a)[4],
 // x = hi + lo with hi the nearest number of 11 bits, which is what tf32 holds,
 // and lo the exact rest, of which the tensor core reads another 11 bits. (Cut
 // off instead of rounded, hi leaves a rest of x's own sign, and what the tensor
-// core drops of it adds up: 1.2e-6 instead of 4.3e-7 of the output.) x from
-// 2^128 (1 - 2^-12) on counts as infinite.
+// core drops of it adds up: 1.2e-6 instead of 4.3e-7 of the output.) From
+// 2^128 (1 - 2^-12) on hi is infinite and lo NaN or infinite.
 __device__ __forceinline__ void split_tf32(float x, unsigned& hi, unsigned& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
@@ -145,6 +149,10 @@ template <> __device__ __forceinline__ void split16<__half>(float p0, float p1, 
   hi = *reinterpret_cast<const unsigned*>(&h);
   lo = *reinterpret_cast<const unsigned*>(&l);
 }
+
+__device__ __forceinline__ float value(const float* p) { return *p; }
+__device__ __forceinline__ float value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float value(const __half* p) { return __half2float(*p); }
 
 template <typename T> __device__ __forceinline__ void store1(void* p, long long i, float v);
 template <> __device__ __forceinline__ void store1<float>(void* p, long long i, float v) { ((float*)p)[i] = v; }
@@ -224,9 +232,9 @@ __device__ __forceinline__ float4 remote4(const float* p, int rank) {
 template <typename T>
 __device__ __forceinline__ void store_out(const AttnArgs& a, int row, int head, int d, float (&acc)[4], float sum, float m) {
   using V = at::Vec4<T>;
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const float inv = 1.0f / sum;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] *= inv;
+  for (int e = 0; e < 4; ++e) acc[e] = sum == 0.f ? 0.f : acc[e] * inv;
   *reinterpret_cast<typename V::raw*>((T*)a.out + row * a.ldo + (long long)head * a.hd + d) = V::put(acc);
   if (a.lse && d == 0) a.lse[(long long)row * a.n_q + head] = (m + log2f(sum)) * 0.6931471805599453f;
 }
@@ -601,6 +609,63 @@ __device__ __forceinline__ void attend(const AttnArgs& a, unsigned char* sm, int
           dst[d] = o[mt][n][j + 2 * r];
         }
     }
+  // NaN: the warp's steps again, position by position, a head after another.
+  // Nothing of a head's sums has to be found infinite for it: an infinite value
+  // that met only positive parts is infinite already.
+  bool nan = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float t = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < HD / 16; ++mt) t += o[mt][n][j] + o[mt][n][j + 2];
+      nan |= n * 8 + 2 * q4 + j < heads && t != t;
+    }
+  if (__any_sync(~0u, nan)) {
+    __syncwarp();
+    constexpr int kD = HD / 32;                                   // elements of a head in a lane
+#pragma unroll 1
+    for (int h = 0; h < heads; ++h) {
+      float x[kD], acc[kD], m = -FLT_MAX, sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < kD; ++e) {
+        const int d = lane + 32 * e;
+        x[e] = d < a.hd ? value(qrow + h * a.hd + d) : 0.f;
+        acc[e] = 0.f;
+      }
+#pragma unroll 1
+      for (int i = 0; i < mine * kStep; ++i) {
+        const int t = t0 + (i / kStep * S::warps + warp) * kStep + i % kStep;
+        if (t >= t1) break;                                       // the last step's end
+        const int pi = (int)a.page.div((unsigned)t), page = table[pi];
+        if (page < 0 || page >= a.n_pages) continue;
+        const long long at = page * a.page_stride + (t - pi * a.page_size) * a.token_stride;
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < kD; ++e)
+          if (lane + 32 * e < a.hd) s = fmaf(x[e], value((const T*)kbase + at + lane + 32 * e), s);
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(~0u, s, w);
+        s *= a.scale_log2;
+        if (s > m) {
+          const float f = ex2(m - s);
+          m = s;
+          sum *= f;
+#pragma unroll
+          for (int e = 0; e < kD; ++e) acc[e] *= f;
+        }
+        const float p = ex2(s - m);
+        sum += p;
+#pragma unroll
+        for (int e = 0; e < kD; ++e)
+          if (lane + 32 * e < a.hd) acc[e] = fmaf(p, value((const T*)vbase + at + lane + 32 * e), acc[e]);
+      }
+      if (lane == 0) { jm[warp * S::heads + h] = m; jl[warp * S::heads + h] = sum; }
+#pragma unroll
+      for (int e = 0; e < kD; ++e) jo[(warp * S::heads + h) * HD + lane + 32 * e] = acc[e];
+    }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < heads * (HD / 4); i += S::warps * 32) {
     const int h = i / (HD / 4), d = i % (HD / 4) * 4;

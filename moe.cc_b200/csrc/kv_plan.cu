@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kMaxSeqs = 16384;      // 12 bytes of shared memory each
 constexpr int kMaxThreads = 512;
+constexpr size_t kStatic = 2 * 32 * sizeof(int);   // the kernel's own shared memory, which counts too
 
 struct PlanArgs {
   const int *past_len, *new_len, *free_pages, *free_head;
@@ -63,6 +64,7 @@ __global__ void __launch_bounds__(kMaxThreads) kv_plan_kernel(const PlanArgs a) 
   pdl_launch();
   extern __shared__ int sm[];
   __shared__ int warp_rows[32], warp_pages[32];
+  static_assert(sizeof(warp_rows) + sizeof(warp_pages) == kStatic, "");
   int *past = sm, *row_end = sm + a.n_seq, *page_end = sm + 2 * a.n_seq;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = gridDim.x, cta = blockIdx.x;
@@ -210,7 +212,7 @@ extern "C" int moe_kv_plan_dev(const int* past_len, const int* new_len, int n_se
   const int ctas = work <= 2 * kMaxThreads ? 1 : work / each < 148 ? (work + each - 1) / each : 148;
   const bool in_place = ctas > 1 && ((kv_len && (kv_len == past_len || kv_len == new_len)) || (free_head_out && free_head_out == free_head));
   const size_t smem = sizeof(int) * 3 * (size_t)n_seq;
-  if (smem > 48 * 1024) {
+  if (smem + kStatic > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)(sizeof(int) * 3 * kMaxSeqs));
     if (e != cudaSuccess) return at::fail(MOE_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));

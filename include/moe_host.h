@@ -130,7 +130,9 @@ int mh_ep_connect(MhModel* m, const void* handles);
  * path (fp32 position * inverse frequency). The attention's sums run in another
  * order and, with 16 bits, over rounded queries, keys and values, so logits are
  * close to the CPU path's but not equal bit for bit. Before the first tokens
- * (position 0); frees the host caches. head_dim a multiple of 8 up to 256
+ * (position 0), also again with another type or page size; frees the host
+ * caches. A call that finds no memory leaves the model on the CPU's (empty)
+ * caches, whichever it had. head_dim a multiple of 8 up to 256
  * (MOE_ERR_UNSUPPORTED otherwise). The device current at the call is used. */
 int mh_kv_device(MhModel* m, int dtype, int page_size);
 

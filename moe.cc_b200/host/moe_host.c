@@ -314,6 +314,20 @@ static void rope_row(float* h, const float* inv_freq, int d2, float p) {
 
 /* ---- model ------------------------------------------------------------------ */
 
+/* The CPU's KV caches, which mh_kv_device frees: there again for a model that
+   comes back to them (empty) because a later mh_kv_device found no memory. */
+static int host_caches(MhModel* m) {
+  if (m->kc) return MOE_OK;
+  const size_t bytes = sizeof(float) * (size_t)m->c.n_layers * m->batch * m->max_ctx * m->Dkv;
+  m->kc = (float*)malloc(bytes);
+  m->vc = (float*)malloc(bytes);
+  if (m->kc && m->vc) return MOE_OK;
+  free(m->kc);
+  free(m->vc);
+  m->kc = m->vc = NULL;
+  return fail(MOE_ERR_NOMEM, "out of host memory (KV cache %zu bytes)", 2 * bytes);
+}
+
 MhModel* mh_create(const MhConfig* cfg, int batch, int max_ctx, int moe_layer_base) {
   if (!cfg || batch < 1 || max_ctx < 1 || cfg->n_layers < 1 || cfg->d_model < 1 || cfg->head_dim < 2 ||
       (cfg->head_dim & 1) || cfg->n_q < 1 || cfg->n_kv < 1 || cfg->n_q % cfg->n_kv || cfg->vocab_size < 1) {
@@ -329,17 +343,15 @@ MhModel* mh_create(const MhConfig* cfg, int batch, int max_ctx, int moe_layer_ba
   m->Dq = cfg->n_q * cfg->head_dim;
   m->Dkv = cfg->n_kv * cfg->head_dim;
   m->layers = (Layer*)calloc((size_t)cfg->n_layers, sizeof(Layer));
-  const size_t kv = (size_t)cfg->n_layers * batch * max_ctx * m->Dkv;
-  m->kc = (float*)malloc(sizeof(float) * kv);
-  m->vc = (float*)malloc(sizeof(float) * kv);
   m->n_threads = omp_get_max_threads();
   m->scores = (float*)malloc(sizeof(float) * (size_t)m->n_threads * max_ctx);
   m->inv_freq = (float*)malloc(sizeof(float) * (size_t)(cfg->head_dim / 2));
   m->moe_ms = (double*)calloc((size_t)cfg->n_layers, sizeof(double));
   m->moe_calls = (long*)calloc((size_t)cfg->n_layers, sizeof(long));
-  if (!m->layers || !m->kc || !m->vc || !m->scores || !m->inv_freq || !m->moe_ms || !m->moe_calls) {
+  if (host_caches(m)) { mh_free(m); return NULL; }
+  if (!m->layers || !m->scores || !m->inv_freq || !m->moe_ms || !m->moe_calls) {
     mh_free(m);
-    fail(MOE_ERR_NOMEM, "mh_create: out of host memory (KV cache %zu bytes)", 2 * sizeof(float) * kv);
+    fail(MOE_ERR_NOMEM, "mh_create: out of host memory");
     return NULL;
   }
   for (int i = 0; i < cfg->head_dim / 2; ++i) {
@@ -688,7 +700,7 @@ int mh_attention(MhModel* m, int layer, const float* x, int T, float* x_after, f
     const int back = kv_enter(m);
     if ((rc = kv_leave(m, back, kv_rows(m, R)))) return rc;
     q = m->h_qkv; k = q + (size_t)R * Dq; v = k + (size_t)R * Dkv;
-  }
+  } else if ((rc = host_caches(m))) return rc;
   rmsnorm_rows(x, w->rms1_w, R, D, eps, m->xn1);
   mm_f32(m->xn1, w->Wq, q, R, Dq, D);
   mm_f32(m->xn1, w->Wk, k, R, Dkv, D);
@@ -1186,6 +1198,7 @@ int mh_fill_kv(MhModel* m, int ctx, uint64_t seed, float std) {
     const int back = kv_enter(m);
     return kv_leave(m, back, kv_fill(m, ctx, seed, std));
   }
+  if ((rc = host_caches(m))) return rc;
   CUDA_OK(cudaMalloc((void**)&tmp, sizeof(float) * row), "device staging");
   for (int l = 0; l < m->c.n_layers; ++l)
     for (int b = 0; b < m->batch; ++b)

@@ -665,8 +665,10 @@ int mh_kv_device(MhModel* m, int dtype, int page_size) {
               (e = cudaMalloc((void**)&m->d_free, sizeof(int) * entries)) ||
               (e = cudaMalloc((void**)&m->d_len, sizeof(int) * 2 * (size_t)m->batch)) ||
               (e = cudaStreamCreateWithFlags(&m->kv_stream, cudaStreamNonBlocking)) ||
-              (e = cudaMemset(m->d_table, 0xff, sizeof(int) * entries)) ||
-              (e = cudaMemcpy(m->d_rope, rope, sizeof(float) * (size_t)m->max_ctx * hd, cudaMemcpyHostToDevice))))
+              /* on the stream that reads them, which the legacy stream does not order */
+              (e = cudaMemsetAsync(m->d_table, 0xff, sizeof(int) * entries, m->kv_stream)) ||
+              (e = cudaMemcpyAsync(m->d_rope, rope, sizeof(float) * (size_t)m->max_ctx * hd, cudaMemcpyHostToDevice, m->kv_stream)) ||
+              (e = cudaStreamSynchronize(m->kv_stream))))
     rc = fail(e == cudaErrorMemoryAllocation ? MOE_ERR_NOMEM : MOE_ERR_CUDA, "mh_kv_device (2 x %zu bytes of cache): %s", bytes,
               cudaGetErrorString(e));
   free(rope);

@@ -61,3 +61,11 @@ def test_without_host_memory_either_the_calls_say_so(driver):
     no_memory(m.fill_kv, 4, 1)
     driver["host_limit"] = -1
     m.attention(0, X, 3)
+
+
+def test_set_up_is_complete_before_the_caches_are_used(driver):
+    """What mh_kv_device writes is read on a stream that does not wait for the
+    legacy one: nothing may be left on that when the call returns."""
+    m = driver.model(1, 12)
+    m.kv_device(mc.F32, 16)
+    assert driver["unordered"] == 0

@@ -52,6 +52,7 @@ constexpr int kMaxParts = 128;      // runs a row is split into at most
 constexpr int kPiece = 64;          // positions of the shortest run
 constexpr int kDealtRows = 512;     // rows whose work is dealt evenly
 constexpr int kRun = 8;             // pieces of the shortest run of more rows
+constexpr int kRowParts = 16384;    // parts of all of them together
 constexpr int kShort = 32;          // pieces up to which a cluster takes a row
 constexpr int kCluster = 8;         // CTAs of such a cluster at most
 enum { kRuns = 0, kDealt = 1, kClustered = 2 };
@@ -948,8 +949,15 @@ Split split_of(long long items, int rows, int max_kv) {
     return {n > 1 ? kClustered : kRuns, n};
   }
   if (rows > kDealtRows) {
-    const int runs = (pieces - 1) / kRun + 1;
-    return {kRuns, runs < kMaxParts ? runs : kMaxParts};
+    // The more rows, the fewer parts each: they fill the GPU, and a part for
+    // every run of each row's context costs workspace and the second launch
+    // (8192 rows of one prompt, 32 heads of 128: 16 parts 2.2 GB and 7.9 ms, 2
+    // parts 0.27 GB and 6.0 ms; one row of 131072 among 600 short ones: 128 parts
+    // 1.3 GB and 0.62 ms, 27 parts 0.27 GB and 0.26 ms).
+    const int runs = (pieces - 1) / kRun + 1, most = kRowParts / rows;
+    if (most <= 1) return {kRuns, 1};
+    const int n = most < kMaxParts ? most : kMaxParts;
+    return {kRuns, runs < n ? runs : n};
   }
   return {kDealt, pieces < kMaxParts ? pieces : kMaxParts};
 }

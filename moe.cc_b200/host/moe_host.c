@@ -608,8 +608,14 @@ static int kv_attention(MhModel* m, int l, int T) {
     cudaFree(m->d_ws);
     m->d_ws = NULL;
     m->ws_bytes = 0;
-    KV_OK(cudaMalloc(&m->d_ws, need), "attention workspace");
-    m->ws_bytes = need;
+    /* for twice the context, so that it does not grow with every step */
+    size_t room = moe_paged_attention_workspace(R, nq, &c, max_kv > m->max_ctx / 2 ? m->max_ctx : 2 * max_kv);
+    if (room < need || cudaMalloc(&m->d_ws, room) != cudaSuccess) {
+      cudaGetLastError();
+      room = need;
+      KV_OK(cudaMalloc(&m->d_ws, need), "attention workspace");
+    }
+    m->ws_bytes = room;
   }
   if ((rc = moe_paged_attention_dev(m->d_q, m->Dq, &c, m->d_table, m->batch, m->kv_max_pages, seq, pos, R, nq, max_kv,
                                     1.0f / sqrtf((float)hd), m->d_out, m->Dq, NULL, m->d_ws, m->ws_bytes, m->kv_stream)))

@@ -69,3 +69,33 @@ def test_set_up_is_complete_before_the_caches_are_used(driver):
     m = driver.model(1, 12)
     m.kv_device(mc.F32, 16)
     assert driver["unordered"] == 0
+
+
+def test_workspace_grows_in_few_steps(driver):
+    """A context that grows token by token: the attention's workspace is
+    allocated anew for twice the context, not for each step."""
+    m = driver.model(1, 400)
+    m.kv_device(mc.F32, 16)
+    m.attention(0, X[:1], 1)
+    driver["ws_per_kv"] = 1000
+    before = driver["mallocs"]
+    for _ in range(399):
+        m.advance(1)
+        m.attention(0, X[:1], 1)
+    assert driver["short_ws"] == 0
+    assert 1 <= driver["mallocs"] - before <= 9          # log2 400
+
+
+def test_workspace_of_the_step_alone_where_twice_is_too_much(driver):
+    m = driver.model(1, 400)
+    m.kv_device(mc.F32, 16)
+    m.attention(0, X[:1], 1)
+    m.advance(99)
+    driver["ws_per_kv"], driver["largest_ok"] = 1000, 150_000
+    m.attention(0, X[:1], 1)
+    assert driver["short_ws"] == 0
+    m.advance(100)
+    no_memory(m.attention, 0, X[:1], 1)
+    driver["largest_ok"] = -1
+    m.attention(0, X[:1], 1)
+    assert driver["short_ws"] == 0

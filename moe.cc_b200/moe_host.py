@@ -183,8 +183,9 @@ class HostModel:
     def fill_kv(self, ctx, seed, std=1.0):
         check(lib().mh_fill_kv(self.h, ctx, seed, std))
 
-    def kv_device(self, dtype=mc.BF16, page_size=16):
-        """Caches and attention on the GPU (dtype mc.F32, mc.F16 or mc.BF16)."""
+    def kv_device(self, dtype=mc.F32, page_size=16):
+        """Caches and attention on the GPU. dtype mc.F32, the CPU caches' own, or
+        mc.F16 or mc.BF16: half the bytes, queries, keys and values rounded."""
         check(lib().mh_kv_device(self.h, dtype, page_size))
 
     def timing(self):

@@ -14,6 +14,7 @@ int fake_mallocs, fake_live;    /* cudaMalloc calls, and allocations alive */
 int fake_unordered;             /* operations on the legacy stream since the host last waited for it */
 long fake_ws_per_kv = 0;        /* bytes of attention workspace per position of max_kv */
 int fake_short_ws;              /* attention calls that got less workspace than they need */
+int fake_cache_dtype = -1;      /* of the last attention call */
 long fake_host_limit = -1;      /* bytes that one malloc of the driver may have; -1: any */
 
 static const char* msg = "";
@@ -74,6 +75,7 @@ int moe_paged_attention_dev(const void* q, long long ldq, const MoeKvCache* c, c
                             size_t bytes, void* s) {
   const size_t need = moe_paged_attention_workspace(rows, nq, c, max_kv);
   if (need && (!ws || bytes < need)) ++fake_short_ws;
+  fake_cache_dtype = c->dtype;
   return MOE_OK;
 }
 int moe_synth_normal_dev(uint64_t seed, uint64_t off, size_t n, float std, float* out, void* s) { return MOE_OK; }

@@ -99,3 +99,11 @@ def test_workspace_of_the_step_alone_where_twice_is_too_much(driver):
     driver["largest_ok"] = -1
     m.attention(0, X[:1], 1)
     assert driver["short_ws"] == 0
+
+
+def test_the_type_that_is_not_named_is_the_drivers_own(driver):
+    """fp32, as on the CPU: fewer bits are a caller's choice."""
+    m = driver.model(1, 12)
+    m.kv_device()
+    m.attention(0, X[:2], 2)
+    assert driver["cache_dtype"] == mc.F32

@@ -10,7 +10,7 @@ torch is plumbing for device memory, never part of the computation).
 There is no CPU fallback: if the library is missing or no GPU is present the
 calls fail loudly. The calls of a decode step around the MoE block (kv_plan,
 qk_norm_rope, paged_attention, route) go through a CPython extension instead
-of ctypes.
+of ctypes, where it could be built.
 """
 import ctypes as C
 import importlib.util
@@ -409,7 +409,9 @@ def moe_ffn_ep(layer, x_norm2, x_inout, stream=None):
 # kv_plan, qk_norm_rope, paged_attention and route take torch CUDA tensors and
 # `stream` as the calls above, and live in a CPython extension (py/moe_fast.c,
 # which also documents them): it refuses a tensor of the wrong type, place or
-# layout before its pointer is handed on. It is loaded with the first of them.
+# layout before its pointer is handed on. It is loaded with the first of them;
+# where it was not built (it needs Python's headers) moe_calls.py does the same
+# through ctypes.
 
 _FAST = ("kv_plan", "qk_norm_rope", "paged_attention", "route")
 FAST_PATH = os.path.join(HERE, "_moe_fast.so")
@@ -419,12 +421,13 @@ def __getattr__(name):
     if name not in _FAST:
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
     lib()
-    if not os.path.exists(FAST_PATH):
-        raise MoeError(MOE_ERR_NOT_INIT, f"{FAST_PATH} is not built (run make -C moe.cc_b200 where Python's headers are)")
-    spec = importlib.util.spec_from_file_location("_moe_fast", FAST_PATH)
-    m = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(m)
-    m._set_error(MoeError)
+    if os.path.exists(FAST_PATH):
+        spec = importlib.util.spec_from_file_location("_moe_fast", FAST_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m._set_error(MoeError)
+    else:
+        import moe_calls as m
     for n in _FAST:
         globals()[n] = getattr(m, n)
     return globals()[name]

@@ -268,10 +268,11 @@ extern "C" int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k,
     return at::fail(MOE_ERR_UNSUPPORTED, "%s: 16-bit rows need a cache of their own type", who);
   if (rows < 0 || n_q < 0 || (long long)n_q + 2ll * cache->n_kv > 32768)
     return at::fail(MOE_ERR_INVALID, "%s: rows %d, n_q %d, n_kv %d", who, rows, n_q, cache->n_kv);
-  if (n_q && (!q || !q_out)) return at::fail(MOE_ERR_INVALID, "%s: q and q_out are needed", who);
-  if (row_slot && (!k || !v)) return at::fail(MOE_ERR_INVALID, "%s: row_slot without k and v", who);
   if (rot_dim < 0 || rot_dim > hd || rot_dim % 8)
     return at::fail(MOE_ERR_UNSUPPORTED, "%s: rot_dim %d (multiples of 8 up to head_dim %d)", who, rot_dim, hd);
+  if (rows == 0) return MOE_OK;
+  if (n_q && (!q || !q_out)) return at::fail(MOE_ERR_INVALID, "%s: q and q_out are needed", who);
+  if (row_slot && (!k || !v)) return at::fail(MOE_ERR_INVALID, "%s: row_slot without k and v", who);
   if (rot_dim && (!rope || rope_len < 1 || !row_pos))
     return at::fail(MOE_ERR_INVALID, "%s: a rotation needs rope, rope_len and row_pos", who);
   if (!(eps >= 0.f)) return at::fail(MOE_ERR_INVALID, "%s: eps must not be negative", who);
@@ -284,7 +285,7 @@ extern "C" int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k,
     return at::fail(MOE_ERR_INVALID, "%s: rows of k and v must start on 16-byte boundaries", who);
   if ((uintptr_t)q_norm % 16 || (uintptr_t)k_norm % 16 || (rot_dim && (uintptr_t)rope % 16))
     return at::fail(MOE_ERR_INVALID, "%s: norm weights and rope must be 16-byte aligned", who);
-  if (rows == 0 || (n_q == 0 && !row_slot)) return MOE_OK;
+  if (n_q == 0 && !row_slot) return MOE_OK;
   // q_out may be q itself; any other overlap would be read after it was written
   const long long nq = (long long)n_q * hd, nk = (long long)cache->n_kv * hd;
   const bool same = q_out == q && ldo == ldq && es == eo;

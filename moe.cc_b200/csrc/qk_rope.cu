@@ -291,7 +291,7 @@ extern "C" int moe_qk_norm_rope_dev(const void* q, long long ldq, const void* k,
   const bool same = q_out == q && ldo == ldq && es == eo;
   if (n_q && !same && at::overlap(q_out, ldo, nq, eo, q, ldq, nq, es, rows))
     return at::fail(MOE_ERR_INVALID, "%s: q_out overlaps q without being q", who);
-  if (n_q && !same && row_slot &&
+  if (n_q && row_slot &&
       (at::overlap(q_out, ldo, nq, eo, k, ldk, nk, es, rows) || at::overlap(q_out, ldo, nq, eo, v, ldv, nk, es, rows)))
     return at::fail(MOE_ERR_INVALID, "%s: q_out overlaps k or v", who);
   at::OnDeviceOf on;

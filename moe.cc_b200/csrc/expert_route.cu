@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kWarps * 32) expert_route_kernel(const RouteAr
 
 template <typename T, int EPL>
 cudaError_t launch_route_epl(const RouteArgs& a, cudaStream_t st) {
-  const unsigned grid = (unsigned)((a.rows + kWarps - 1) / kWarps);
+  const unsigned grid = ((unsigned)a.rows + kWarps - 1) / kWarps;
   const size_t smem = a.groups > 1 ? sizeof(double) * kWarps * EPL * 32 : 0;
   if (a.bias) return launch_pdl(expert_route_kernel<T, EPL, kByScore>, dim3(grid), dim3(kWarps * 32), smem, st, a);
   if (a.groups > 1) return launch_pdl(expert_route_kernel<T, EPL, kByGroup>, dim3(grid), dim3(kWarps * 32), smem, st, a);

@@ -228,7 +228,7 @@ cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
     // as much as a few of its heads: with 2 or 4 warps a row, 4096 rows took
     // 26 and 34 us where one a row took 23.)
     const int per = 32 / lph, groups = (a.n_q + per - 1) / per + (a.row_slot ? 2 * ((a.n_kv + per - 1) / per) : 0);
-    const long long want = (3552 + a.rows - 1) / a.rows;
+    const long long want = (3551ll + a.rows) / a.rows;
     a.per_row = (int)(want < groups ? want : groups);
     const long long blocks = ((long long)a.rows * a.per_row + kWarps - 1) / kWarps;
     return launch_pdl(kernel, dim3((unsigned)blocks), dim3(kWarps * 32), 0, st, a);

@@ -25,8 +25,10 @@
 // One warp routes one token: expert j * 32 + lane in lane `lane`. A round of
 // the selection takes the largest key by a warp reduction, then the lowest
 // index that has it by another; 16-bit logits carry the index in the key's
-// other half and need one. Issue slots are the bound: a token costs a few
-// hundred instructions a warp, its logits a few hundred bytes.
+// other half and need one. Its logits are a few hundred bytes; the bound is
+// instructions: issue slots where tokens are many (16384 of 128 experts: 77 %
+// of them busy), the chain of one warp where they are less than a wave (4096 of
+// 256 with groups and bias: 48 % busy, 36 % of the warps active, 9.8 us).
 #include "attn.cuh"
 
 #include <type_traits>

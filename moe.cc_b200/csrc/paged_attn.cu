@@ -132,7 +132,7 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], const unsigned (&a)[4],
 // x = hi + lo with hi the nearest number of 11 bits, which is what tf32 holds,
 // and lo the exact rest, of which the tensor core reads another 11 bits. (Cut
 // off instead of rounded, hi leaves a rest of x's own sign, and what the tensor
-// core drops of it adds up: 1.2e-6 instead of 4.3e-7 of the output.) From
+// core drops of it adds up: 1.2e-6 instead of 4 to 5e-7 of the output.) From
 // 2^128 (1 - 2^-12) on hi is infinite and lo NaN or infinite.
 __device__ __forceinline__ void split_tf32(float x, unsigned& hi, unsigned& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;

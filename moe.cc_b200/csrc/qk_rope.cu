@@ -223,10 +223,11 @@ __global__ void __launch_bounds__(kWarps * 32, 8) qk_norm_rope_kernel(const Rope
 template <typename TI, typename TO>
 cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
   auto go = [&](auto kernel, int lph) {
-    // One warp a row where that fills the GPU (24 warps an SM), else more, up
-    // to one for each group of heads. (A row's table entries and weights cost
-    // as much as a few of its heads: with 2 or 4 warps a row, 4096 rows took
-    // 26 and 34 us where one a row took 23.)
+    // One warp a row from 3552 rows on (24 warps an SM; registers let 16 be
+    // resident, so 4096 rows are 1.7 waves), else more, up to one for each group
+    // of heads. (A row's table entries and weights cost as much as a few of its
+    // heads: with 2 or 4 warps a row, 4096 rows took 26 and 34 us where one a
+    // row took 23.)
     const int per = 32 / lph, groups = (a.n_q + per - 1) / per + (a.row_slot ? 2 * ((a.n_kv + per - 1) / per) : 0);
     const long long want = (3551ll + a.rows) / a.rows;
     a.per_row = (int)(want < groups ? want : groups);

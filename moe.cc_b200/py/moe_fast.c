@@ -3,8 +3,8 @@
  * paged_attention, route of moe_cuda.py) as a CPython extension.
  *
  * These calls run kernels of 2 to 5 us. Checked and handed on by Python and
- * ctypes they took the host 6 to 16 us, most of it for reading the tensors'
- * attributes and converting 20 arguments; from here they take 4 to 13.
+ * ctypes (moe_calls.py) they take the host 9 to 20 us, most of it for reading the
+ * tensors' attributes and converting 20 arguments; from here they take 4 to 13.
  * Each tensor's type, device, shape and layout is checked before its pointer
  * goes on; a wrong one raises moe_cuda.MoeError, as an error of the library
  * does. torch is not linked: tensors are read through their Python attributes.
